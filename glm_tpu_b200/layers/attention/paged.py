@@ -1,0 +1,141 @@
+"""Attention over a paged cache for a few drafted tokens per sequence, and the append that fills the cache.
+
+A step over drafted tokens: ``append`` normalizes and rotates the rows of a fused ``q | k | v`` projection and writes keys and values into the slots behind
+each sequence's committed ones; ``tree_attention`` lets every drafted token see the committed slots and its ancestors.  ``ancestor_masks`` makes the masks
+of a tree.  Tokens that were accepted are appended once more, at consecutive slots (their position, and so their rotation, stays): rows of one call
+are read from the projection and not from the cache, so no slot is moved within it.  A tree of one token is ordinary decoding, a chain a short prompt.
+
+bf16, fp32 sums, one rounding of every result.  Sequences, slots, pages and positions out of range are never followed: they are OR-ed into ``status`` (an
+int32 tensor of one element on the same GPU) as a bad index, the row stores nothing and its queries are zeros; in attention such a slot is not attended to.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Sequence
+from dataclasses import dataclass
+
+import torch
+
+from glm_tpu_b200.oracle import scoring
+
+MAX_DRAFTS = 64
+MAX_SLOTS = 1 << 30
+
+
+@dataclass(frozen=True)
+class PagedKV:
+    """A pool of pages and the table that says which of them hold a sequence's slots: slot ``s`` of sequence ``b`` is row ``s % page`` of page
+    ``table[b, s // page]``.  Entries behind a sequence's last page may hold anything."""
+
+    k: torch.Tensor  # [pages, page, kv_heads, dim] bf16, heads' channels contiguous
+    v: torch.Tensor  # [pages, page, kv_heads, vdim]
+    table: torch.Tensor  # [sequences, pages of a sequence] int32
+
+
+def ancestor_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
+    """Masks (int64) and depths (int32) of a drafted tree on the CPU: ``parents[j] < j`` is the drafted token that token ``j`` follows, -1 the last
+    committed one.  Bit ``i`` of ``masks[j]``: token ``i`` is ``j`` or one of its ancestors.  A token's position is the committed length + its depth."""
+    if len(parents) > MAX_DRAFTS or any(not -1 <= p < j for j, p in enumerate(parents)):
+        raise ValueError(f"up to {MAX_DRAFTS} drafted tokens, each behind its parent")
+    masks, depths = [], []
+    for j, p in enumerate(parents):
+        masks.append((masks[p] if p >= 0 else 0) | 1 << j)
+        depths.append(depths[p] + 1 if p >= 0 else 0)
+    return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64), torch.tensor(depths, dtype=torch.int32)
+
+
+def _check_cache(cache: PagedKV, device: torch.device) -> None:
+    k, v, table = cache.k, cache.v, cache.table
+    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.shape[1] or not k.shape[2]:
+        raise ValueError("pools are [pages, page, kv_heads, dim] and [pages, page, kv_heads, vdim] in bf16")
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1) or table.shape[1] * k.shape[1] > MAX_SLOTS:
+        raise ValueError("the table is [sequences, pages of a sequence] in int32, of up to 2^30 slots a sequence")
+    if k.device != device or v.device != device or table.device != device:
+        raise ValueError("rows, pools and table lie on one device")
+    dim, vdim = k.shape[3], v.shape[3]
+    if not 16 <= dim <= 256 or not 16 <= vdim <= 256 or dim % 16 or vdim % 16:
+        raise ValueError("heads are 16 to 256 channels wide, in multiples of 16")
+    if k.is_cuda and (k.stride(3) != 1 or v.stride(3) != 1 or any(s % 8 for s in (*k.stride()[:3], *v.stride()[:3])) or (k.data_ptr() | v.data_ptr()) % 16):
+        raise ValueError("the channels of a head are contiguous and every head of the pools 16-byte aligned")
+
+
+def _check_index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> None:
+    if t.shape != (n,) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: {n} contiguous elements of {str(dtype)[6:]} on the device of the rows")
+
+
+def append(qkv: torch.Tensor, cache: PagedKV, positions: torch.Tensor | None, seqs: torch.Tensor, slots: torch.Tensor, *, heads: int,
+           rot: torch.Tensor | None = None, pairs: bool = False, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+           want_q: bool = True, status: torch.Tensor | None = None) -> torch.Tensor | None:
+    """``qkv [rows, heads * dim + kv_heads * (dim + vdim)]`` bf16 -> queries ``[rows, heads, dim]``; keys and values into the cache.
+
+    ``rot``: fp32 ``[positions, n, 2]`` (cos, sin) for the leading ``2 n`` channels of q and k, as halves ``(d, d + n)`` or, with ``pairs``, as neighbours
+    ``(2j, 2j + 1)``; ``q_norm`` / ``k_norm``: bf16 ``[dim]``, RMS norm of every head before the rotation.  A negative slot stores nothing.  Rows of one call name different
+    slots.  ``want_q=False``: keys and values only (returns ``None``)."""
+    _check_cache(cache, qkv.device)
+    G, dim, vdim = cache.k.shape[2], cache.k.shape[3], cache.v.shape[3]
+    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or heads < 1 or qkv.shape[1] != heads * dim + G * (dim + vdim):
+        raise ValueError("qkv is [rows, heads * dim + kv_heads * (dim + vdim)] in bf16")
+    rows = qkv.shape[0]
+    _check_index("seqs", seqs, rows, torch.int32, qkv.device)
+    _check_index("slots", slots, rows, torch.int32, qkv.device)
+    if rot is not None:
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+        _check_index("positions", positions, rows, torch.int32, qkv.device)
+        if rot.dim() != 3 or rot.shape[2] != 2 or 2 * rot.shape[1] > dim or not rot.shape[1] or rot.dtype != torch.float32 or not rot.is_contiguous() or rot.device != qkv.device:
+            raise ValueError("rot is [positions, n, 2] in fp32, contiguous, with 2 n channels at most as many as a head has")
+    for weight in (q_norm, k_norm):
+        if weight is not None:
+            _check_index("norm", weight, dim, torch.bfloat16, qkv.device)
+    if not qkv.is_cuda:
+        q = scoring.append(qkv, cache.k, cache.v, cache.table, positions, seqs, slots, heads=heads, q_norm=q_norm, k_norm=k_norm, eps=eps, rot=rot, pairs=pairs)
+        return q if want_q else None
+    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+        raise ValueError("rows of qkv are contiguous and 16-byte aligned")
+    from glm_tpu_b200.ops import native
+
+    with torch.cuda.device(qkv.device):
+        q = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=qkv.device) if want_q else None
+        native.paged_append(qkv, cache.k, cache.v, cache.table, positions, seqs, slots, q, heads, rot, pairs, q_norm, k_norm, eps, status=status)
+    return q
+
+
+def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, lengths: torch.Tensor, masks: torch.Tensor, scale: float, *, max_rows: int,
+                   sink: torch.Tensor | None = None, out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``q [rows, heads, dim]`` bf16 -> ``[rows, heads, vdim]``.
+
+    Sequence ``b`` owns rows ``starts[b] .. starts[b + 1] - 1`` (int32, ascending), ``lengths[b]`` (int32) committed slots, and its drafted tokens lie in the slots behind
+    those, one per row in order.  ``masks`` (int64): bit ``t`` lets a row see its sequence's drafted slot ``t``; bits of rows that the sequence does
+    not have mean nothing.  ``max_rows`` (at most 64): rows of the largest sequence.  ``sink``: fp32 ``[heads]``, a score that takes weight and gives no value.  A row
+    that sees nothing, without a sink, is zeros.  Rows that belong to no sequence stay as they are in ``out``, or are zeros where it is made here."""
+    _check_cache(cache, q.device)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != cache.k.shape[3] or not q.shape[1] or q.shape[1] % cache.k.shape[2]:
+        raise ValueError("q is [rows, heads, dim] in bf16, with a multiple of the cache's heads")
+    rows, heads, _ = q.shape
+    seqs, vdim = cache.table.shape[0], cache.v.shape[3]
+    if seqs > 65535:
+        raise ValueError("at most 65,535 sequences")
+    _check_index("starts", starts, seqs + 1, torch.int32, q.device)
+    _check_index("lengths", lengths, seqs, torch.int32, q.device)
+    _check_index("masks", masks, rows, torch.int64, q.device)
+    if not 1 <= max_rows <= MAX_DRAFTS:
+        raise ValueError(f"between 1 and {MAX_DRAFTS} rows a sequence")
+    if sink is not None:
+        _check_index("sink", sink, heads, torch.float32, q.device)
+    if out is not None and (out.shape != (rows, heads, vdim) or out.dtype != torch.bfloat16 or out.device != q.device):
+        raise ValueError("out is [rows, heads, vdim] in bf16 on the device of q")
+    if not q.is_cuda:
+        out = torch.zeros((rows, heads, vdim), dtype=torch.bfloat16) if out is None else out
+        return scoring.tree_attention(q, cache.k, cache.v, cache.table, starts, lengths, masks, scale, max_rows, sink, out)
+    for t in (q, out):
+        if t is not None and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+            raise ValueError("the channels of a head are contiguous and every head of q and out 16-byte aligned")
+    from glm_tpu_b200.ops import native
+
+    with torch.cuda.device(q.device):
+        made = out is None
+        if made:
+            out = (torch.empty if seqs else torch.zeros)((rows, heads, vdim), dtype=torch.bfloat16, device=q.device)
+        native.tree_attention(q, cache.k, cache.v, cache.table, starts, lengths, masks, scale, max_rows, sink, out, clear_rest=made, status=status)
+    return out

@@ -26,3 +26,14 @@ class SelectedPositions:
 class RouterOutput:
     expert_ids: torch.Tensor  # [rows, top_k] int32, descending choice score, ties to the lowest expert id
     weights: torch.Tensor  # [rows, top_k] fp32, normalized unbiased sigmoid scores (the routed scale is applied later)
+
+
+@dataclass
+class TokenLogprobs:
+    """What ``layers.logprobs`` says of every row; natural logarithms, fp32."""
+
+    logprob: torch.Tensor  # [rows] of the given token
+    entropy: torch.Tensor  # [rows] of the row's distribution
+    best: torch.Tensor  # [rows] of the most likely token
+    top_ids: torch.Tensor | None  # [rows, top] int32, most likely first, ties to the lowest id
+    top_logprobs: torch.Tensor | None  # [rows, top]

@@ -135,9 +135,50 @@ class DeltaArgs(C.Structure):
     ]
 
 
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("stride", C.c_int64), ("tokens", C.c_void_p),
+        ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("best", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
+        ("rows", C.c_int), ("vocab", C.c_int), ("top", C.c_int), ("is_f32", C.c_int), ("tokens_64", C.c_int),
+        ("status", C.c_void_p),
+    ]
+
+
+class PagedArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("k_page", C.c_int64), ("k_slot", C.c_int64), ("k_head", C.c_int64),
+        ("v", C.c_void_p), ("v_page", C.c_int64), ("v_slot", C.c_int64), ("v_head", C.c_int64),
+        ("table", C.c_void_p), ("table_stride", C.c_int64),
+        ("seqs", C.c_int), ("per_seq", C.c_int), ("pages", C.c_int), ("page", C.c_int), ("G", C.c_int), ("dim", C.c_int), ("vdim", C.c_int),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedArgs),
+        ("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+        ("rot", C.c_void_p), ("rot_dims", C.c_int), ("rot_rows", C.c_int), ("pairs", C.c_int),
+        ("positions", C.c_void_p), ("row_seq", C.c_void_p), ("slots", C.c_void_p),
+        ("q", C.c_void_p), ("q_stride", C.c_int64), ("rows", C.c_int), ("H", C.c_int), ("eps", C.c_float),
+        ("status", C.c_void_p),
+    ]
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedArgs),
+        ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64),
+        ("starts", C.c_void_p), ("lengths", C.c_void_p), ("masks", C.c_void_p), ("sink", C.c_void_p),
+        ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("splits", C.c_int),
+        ("rows", C.c_int), ("H", C.c_int), ("max_rows", C.c_int), ("scale", C.c_float), ("clear_rest", C.c_int),
+        ("status", C.c_void_p),
+    ]
+
+
 # argument structures and the entry point that gives their size in the library
 _STRUCTS = (("glmb_qkv_conv_args_sizeof", QkvConvArgs), ("glmb_chunk_attn_args_sizeof", ChunkAttnArgs), ("glmb_latent_args_sizeof", LatentArgs),
-            ("glmb_delta_args_sizeof", DeltaArgs))
+            ("glmb_delta_args_sizeof", DeltaArgs), ("glmb_token_logprobs_args_sizeof", TokenLogprobsArgs),
+            ("glmb_paged_append_args_sizeof", PagedAppendArgs), ("glmb_tree_attention_args_sizeof", TreeAttentionArgs))
 
 _lib = None
 
@@ -823,6 +864,66 @@ def step_finalize(cand, n_sets, rows, row_active, tokens, positions, out_tokens,
                                  _p(positions), _p(out_tokens), _p(step_counter), ring, int(advance), _comm(comm), sig, _stream()),
         "step_finalize",
     )
+
+
+# ----------------------------------------------------------------------------- log probabilities of given tokens
+def token_logprobs(logits, tokens, sums, top_ids=None, top_logprobs=None, *, status=None):
+    """``sums`` fp32 ``[3, rows]``: log probability of ``tokens`` (int32 or int64), entropy, log probability of the most likely token; with ``top_ids``
+    int32 and ``top_logprobs`` fp32 ``[rows, top]`` the most likely tokens, ties to the lowest id.  bf16 or fp32 logits, one pass."""
+    rows, vocab = logits.shape
+    out, item = sums.data_ptr(), 4 * rows
+    a = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0), tokens.data_ptr(), out, out + item, out + 2 * item,
+                          None if top_ids is None else top_ids.data_ptr(), None if top_logprobs is None else top_logprobs.data_ptr(),
+                          rows, vocab, 0 if top_ids is None else top_ids.shape[1], logits.dtype == torch.float32, tokens.dtype == torch.int64,
+                          None if status is None else status.data_ptr())
+    _check(lib().glmb_token_logprobs(C.byref(a), _stream()), "token_logprobs")
+
+
+HEAD_SLAB = 1 << 26  # logits of a slab of rows
+
+
+def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
+    """``token_logprobs`` of ``hidden @ head[:vocab].T``, some rows at a time."""
+    rows = hidden.shape[0]
+    step = max(1, min(rows, HEAD_SLAB // head.shape[0]))
+    padded = -(-head.shape[0] // 8) * 8
+    logits = torch.empty((step, padded), dtype=torch.float32, device=hidden.device)
+    for r in range(0, rows, step):
+        n = min(step, rows - r)
+        part = torch.empty((3, n), dtype=torch.float32, device=hidden.device)
+        if hidden.dtype == torch.float32:
+            gemm_f32(hidden[r : r + n], head, logits[:n])
+        else:
+            for i in range(0, n, MAX_ROWS):
+                skinny_bf16(hidden[r + i : r + min(n, i + MAX_ROWS)], head, logits[i:n], SK_OUT_F32)
+        token_logprobs(logits[:n, :vocab], tokens[r : r + n], part, status=status)
+        sums[:, r : r + n] = part
+
+
+# ----------------------------------------------------------------------------- drafted tokens over a paged cache
+def _paged(k, v, table) -> PagedArgs:
+    pages, page, G, dim = k.shape
+    ks, vs = k.stride(), v.stride()
+    return PagedArgs(k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], pages, page,
+                     G, dim, v.shape[3])
+
+
+def paged_append(qkv, k, v, table, positions, seqs, slots, q, heads, rot=None, pairs=False, q_norm=None, k_norm=None, eps=1e-6, *, status=None):
+    """Norm and rotation of the heads of a fused projection; keys and values into the pages of their slots (``layers.attention.paged.append``)."""
+    a = PagedAppendArgs(_paged(k, v, table), qkv.data_ptr(), qkv.stride(0), None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                        None if rot is None else rot.data_ptr(), 0 if rot is None else 2 * rot.shape[1], 0 if rot is None else rot.shape[0], int(pairs),
+                        None if positions is None else positions.data_ptr(), seqs.data_ptr(), slots.data_ptr(), None if q is None else q.data_ptr(),
+                        heads * k.shape[3], qkv.shape[0], heads, eps, None if status is None else status.data_ptr())
+    _check(lib().glmb_paged_append(C.byref(a), _stream()), "paged_append")
+
+
+def tree_attention(q, k, v, table, starts, lengths, masks, scale, max_rows, sink, out, *, clear_rest=False, status=None):
+    """Attention of drafted rows over a paged cache and their ancestors (``layers.attention.paged.tree_attention``)."""
+    rows, H, _ = q.shape
+    a = TreeAttentionArgs(_paged(k, v, table), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), starts.data_ptr(), lengths.data_ptr(),
+                          masks.data_ptr(), None if sink is None else sink.data_ptr(), None, None, 1, rows, H, max_rows, scale, int(clear_rest),
+                          None if status is None else status.data_ptr())
+    _check(lib().glmb_tree_attention(C.byref(a), _stream()), "tree_attention")
 
 
 def fp8_to_bf16(bits, scale, out, block=(128, 128), status=None):
