@@ -135,12 +135,19 @@ class DeltaArgs(C.Structure):
     ]
 
 
+class TokenScores(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("best", C.c_void_p), ("tokens_64", C.c_int),
+        ("status", C.c_void_p),
+    ]
+
+
 class TokenLogprobsArgs(C.Structure):
     _fields_ = [
-        ("logits", C.c_void_p), ("stride", C.c_int64), ("tokens", C.c_void_p),
-        ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("best", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
-        ("rows", C.c_int), ("vocab", C.c_int), ("top", C.c_int), ("is_f32", C.c_int), ("tokens_64", C.c_int),
-        ("status", C.c_void_p),
+        ("logits", C.c_void_p), ("stride", C.c_int64),
+        ("scores", TokenScores),
+        ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
+        ("rows", C.c_int), ("vocab", C.c_int), ("top", C.c_int), ("is_f32", C.c_int),
     ]
 
 
@@ -867,15 +874,17 @@ def step_finalize(cand, n_sets, rows, row_active, tokens, positions, out_tokens,
 
 
 # ----------------------------------------------------------------------------- log probabilities of given tokens
+def _scores(tokens, sums, status) -> TokenScores:
+    out, item = sums.data_ptr(), sums.stride(0) * 4
+    return TokenScores(tokens.data_ptr(), out, out + item, out + 2 * item, tokens.dtype == torch.int64, None if status is None else status.data_ptr())
+
+
 def token_logprobs(logits, tokens, sums, top_ids=None, top_logprobs=None, *, status=None):
     """``sums`` fp32 ``[3, rows]``: log probability of ``tokens`` (int32 or int64), entropy, log probability of the most likely token; with ``top_ids``
     int32 and ``top_logprobs`` fp32 ``[rows, top]`` the most likely tokens, ties to the lowest id.  bf16 or fp32 logits, one pass."""
     rows, vocab = logits.shape
-    out, item = sums.data_ptr(), 4 * rows
-    a = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0), tokens.data_ptr(), out, out + item, out + 2 * item,
-                          None if top_ids is None else top_ids.data_ptr(), None if top_logprobs is None else top_logprobs.data_ptr(),
-                          rows, vocab, 0 if top_ids is None else top_ids.shape[1], logits.dtype == torch.float32, tokens.dtype == torch.int64,
-                          None if status is None else status.data_ptr())
+    a = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0), _scores(tokens, sums, status), None if top_ids is None else top_ids.data_ptr(),
+                          None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab, 0 if top_ids is None else top_ids.shape[1], logits.dtype == torch.float32)
     _check(lib().glmb_token_logprobs(C.byref(a), _stream()), "token_logprobs")
 
 
@@ -890,14 +899,12 @@ def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
     logits = torch.empty((step, padded), dtype=torch.float32, device=hidden.device)
     for r in range(0, rows, step):
         n = min(step, rows - r)
-        part = torch.empty((3, n), dtype=torch.float32, device=hidden.device)
         if hidden.dtype == torch.float32:
             gemm_f32(hidden[r : r + n], head, logits[:n])
         else:
             for i in range(0, n, MAX_ROWS):
                 skinny_bf16(hidden[r + i : r + min(n, i + MAX_ROWS)], head, logits[i:n], SK_OUT_F32)
-        token_logprobs(logits[:n, :vocab], tokens[r : r + n], part, status=status)
-        sums[:, r : r + n] = part
+        token_logprobs(logits[:n, :vocab], tokens[r : r + n], sums[:, r : r + n], status=status)
 
 
 # ----------------------------------------------------------------------------- drafted tokens over a paged cache
