@@ -39,7 +39,7 @@ struct TreeAttentionArgs {
     bf16* out; int64_t out_row, out_head;
     const int* starts; const int* lengths; const int64_t* masks;
     const float* sink;
-    float* part_o; float* part_ml; int splits;
+    float* part_o; float* part_ml; int64_t parts;  // room for so many sums (vdim floats, and 2)
     int rows, H, max_rows;
     float scale;
     int clear_rest;  // rows behind the last sequence become zeros (a buffer that nobody wrote), else they stay as they are

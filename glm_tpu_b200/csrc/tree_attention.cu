@@ -1,20 +1,53 @@
-// Attention of a few drafted tokens per sequence over a paged cache (bf16; scores, softmax and sums fp32).
+// Attention of a few drafted tokens per sequence over a paged cache (bf16) on the 5th-generation tensor cores.
 //
 // Row j of a sequence, whose committed tokens lie in slots 0 .. length - 1 and whose drafted tokens in slots length, length + 1, ..:
 //
 //   o = sum_i p_i v_i,   p_i = e^(scale q . k_i) / (sum e^(scale q . k) + e^sink)
 //
 // over every committed slot and the drafted slots t (those of this call's rows) with bit t of the row's mask: its ancestors in the tree and itself.
-// What a row does not attend to is never multiplied, so NaN there stays there.  Nothing attended: zeros.  A slot whose page the table does not know
-// counts as not attended and raises GLMB_STATUS_BAD_INDEX, as does a sequence whose rows or length are out of range.
+// A row that sees nothing gives zeros.  A slot whose page the table does not know counts as not attended and raises GLMB_STATUS_BAD_INDEX, as does a
+// sequence whose rows or length are out of range.
+//
+// A tile is up to 128 (drafted row, head) pairs of one key head: the M of both products.  A unit is a sequence's key head with one tile, or with two that
+// take turns on the tensor core; its keys come in blocks of 128.  The blocks of all units, one after another, are dealt to one CTA per SM in equal runs, so
+// that unequal sequences keep every SM streaming; a run may begin and end inside a unit.  For each block of a tile:
+//
+//   S = Q K^T       both operands K-major in shared memory (TMA, 128-byte swizzle), fp32 scores in TMEM
+//   softmax         128 threads, one row each, running maximum and sum in fp32; weights back into TMEM where the scores were, in bf16
+//   O += P V        A = weights from TMEM, B = values as they lie in memory
+//
+// The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
+// (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-9 beside that of the result.
+// A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; memory is its bound, so its weights
+// keep a second piece, the remainder of the first.  Heads wider than 128 (WIDE): blocks of 64 keys, one group.
+//
+//   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
+//   warp 8           issues every tcgen05.mma, owns the TMEM allocation
+//   warp 9           looks pages up, brings queries, keys and values in by TMA
+//
+// What a row does not see must not reach it, and a weight of zero times NaN is NaN.  Slots behind the last one, and pages that do not exist, are read as zeros
+// (out of the tensor map's range) or cleared in shared memory before the product; drafted values that are not finite are cleared too, and the rows
+// that do see them add their product afterwards, one by one.
+//
+// Runs that share a unit leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.
+// Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
 #include "paged.cuh"
+#include "tcgen05.cuh"
 #include "vec8.cuh"
 
 #define TA_LOG2E 1.4426950408889634f
 #define TA_MAX_DRAFTS 64  // bits of a mask
+#define TA_THREADS 320
+#define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
+#define TA_NOTES 8        // blocks whose pages are remembered: the producer is at most five ahead of the softmax
+
+enum { TA_PAIR = 0, TA_SINGLE = 1, TA_WIDE = 2 };
 
 // Rows and committed slots of a sequence, within what there is.
-struct TreeSeq { int row0, rows, length; };
+struct TreeSeq {
+    int row0, rows, drafts, length;
+    __device__ __forceinline__ int blocks(int keys) const { return rows ? (length + drafts + keys - 1) / keys : 0; }
+};
 __device__ __forceinline__ TreeSeq tree_seq(const TreeAttentionArgs& a, int b, bool report) {
     TreeSeq s;
     const int from = a.starts[b], to = a.starts[b + 1], length = a.lengths[b];
@@ -22,83 +55,642 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttentionArgs& a, int b, b
     s.rows = max(min(to, a.rows) - s.row0, 0);
     s.length = min(max(length, 0), a.cache.per_seq * a.cache.page);
     if (report && (from != s.row0 || to < from || to > a.rows || s.rows > a.max_rows || s.length != length)) raise_status(a.status, GLMB_STATUS_BAD_INDEX);
+    s.rows = min(s.rows, a.max_rows);
+    s.drafts = s.rows;
     return s;
 }
 
-// grid (heads, max_rows, sequences); a warp takes every fourth key.
-__global__ void __launch_bounds__(128) tree_attention_kernel(TreeAttentionArgs a) {
-    GLMB_PDL_PROLOGUE();
-    __shared__ float o_s[4][256], ml_s[4][2];
-    const int h = blockIdx.x, j = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const PagedArgs& c = a.cache;
-    const TreeSeq seq = tree_seq(a, b, h == 0 && j == 0 && threadIdx.x == 0);
-    if (a.clear_rest && j == 0) {
-        const int last = b + 1 == c.seqs ? a.rows : seq.row0 + seq.rows, first = seq.row0 + min(seq.rows, a.max_rows);
-        for (int r = b == 0 ? 0 : first; r < last; ++r)
-            if (r < seq.row0 || r >= first)
-                for (int d = threadIdx.x; d < c.vdim; d += 128) a.out[(int64_t)r * a.out_row + (int64_t)h * a.out_head + d] = __float2bfloat16_rn(0.f);
+// How units are made: `heads` of a tile (of `head_blocks` of a key head), `tile_rows` drafted rows of a tile, tiles of a unit.
+struct TreeShape {
+    int per, heads, head_blocks, tile_rows, in_unit, keys, ctas, units_max;  // units_max: of a key head of the largest sequence
+    __device__ __forceinline__ int tiles(int rows) const { return (rows + tile_rows - 1) / tile_rows * head_blocks; }
+    __device__ __forceinline__ int units(int rows) const { return (tiles(rows) + in_unit - 1) / in_unit; }
+};
+
+// Blocks of all sequences before sequence b (`upto` = seqs: all); the whole warp.
+__device__ __forceinline__ int64_t tree_blocks(const TreeAttentionArgs& a, const TreeShape& sh, int upto, int lane) {
+    int64_t sum = 0;
+    for (int b = lane; b < upto; b += 32) {
+        const TreeSeq s = tree_seq(a, b, false);
+        sum += (int64_t)s.blocks(sh.keys) * sh.units(s.rows) * a.cache.G;
     }
-    if (j >= seq.rows) return;
-    const int row = seq.row0 + j, g = h / (a.H / c.G), drafts = min(seq.rows, min(a.max_rows, TA_MAX_DRAFTS));
-    const int64_t mask = a.masks[row];
-    const bf16* q = a.q + (int64_t)row * a.q_row + (int64_t)h * a.q_head;
-    float qv[8], o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        qv[i] = lane + 32 * i < c.dim ? to_f32(q[lane + 32 * i]) : 0.f;
-        o[i] = 0.f;
-    }
-    const float scale2 = a.scale * TA_LOG2E;
-    float m = -INFINITY, l = 0.f;
-    for (int s = warp; s < seq.length + drafts; s += 4) {
-        if (s >= seq.length && !((mask >> (s - seq.length)) & 1)) continue;
-        const int page = paged_page(c, b, s);
-        if (page < 0) {
-            if (lane == 0) raise_status(a.status, GLMB_STATUS_BAD_INDEX);
-            continue;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+// The part of a CTA's run that lies in one unit.
+struct TreeSegment {
+    TreeSeq seq;
+    int b, g, unit;       // unit of the sequence's key head
+    int block0, blocks;   // of `of` blocks of the unit
+    int of;
+};
+// Walks a run.
+struct TreeWalk {
+    int64_t left;
+    int b, at;  // the sequence, and how many of its (key head, unit) pairs are done
+    int block0;
+    __device__ __forceinline__ bool next(const TreeAttentionArgs& a, const TreeShape& sh, TreeSegment& s) {
+        while (left > 0 && b < a.cache.seqs) {
+            s.seq = tree_seq(a, b, false);
+            s.of = s.seq.blocks(sh.keys);
+            const int units = s.of ? sh.units(s.seq.rows) : 0;
+            if (at >= units * a.cache.G) {
+                ++b, at = 0, block0 = 0;
+                continue;
+            }
+            s.b = b, s.g = at / units, s.unit = at % units, s.block0 = block0;
+            s.blocks = (int)min((int64_t)(s.of - block0), left);
+            left -= s.blocks;
+            ++at, block0 = 0;
+            return true;
         }
-        const bf16* k = c.k + page * c.k_page + (s % c.page) * c.k_slot + g * c.k_head;
-        const bf16* v = c.v + page * c.v_page + (s % c.page) * c.v_slot + g * c.v_head;
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < c.dim) dot = fmaf(qv[i], to_f32(k[lane + 32 * i]), dot);
-        const float x = warp_sum(dot) * scale2, next = fmaxf(m, x);
-        const float fix = m == next ? 1.f : exp2f(m - next), p = exp2f(x - next);
-        m = next;
-        l = l * fix + p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < c.vdim) o[i] = o[i] * fix + p * to_f32(v[lane + 32 * i]);
+        return false;
     }
-    if (lane == 0) ml_s[warp][0] = m, ml_s[warp][1] = l;
-    for (int i = 0; i < 8; ++i) o_s[warp][lane + 32 * i] = o[i];
+};
+
+__device__ __forceinline__ void ta_tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void ta_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void ta_tma_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void ta_tma_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// MN-major operand, 128-byte swizzle: 64 columns (128 bytes) per K row, 8 K rows per 1024-byte group, 64-column boxes `box` bytes apart
+__device__ __forceinline__ uint64_t ta_desc_mn(uint32_t smem_addr, uint32_t box) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(box >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ float ta_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Bits i of a word of 32 keys whose first lies `ahead` slots behind the first drafted one (negative: before it): committed, or drafted and in the mask.
+__device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
+    if (ahead >= 64) return 0u;
+    if (ahead >= 0) return (uint32_t)(mask >> ahead);
+    if (ahead <= -32) return ~0u;
+    return (uint32_t)(mask << -ahead) | ((1u << -ahead) - 1u);
+}
+
+template <int MODE> struct TreeMode {
+    static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2;
+    static constexpr int STAGES = MODE == TA_SINGLE ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
+    static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
+    static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + 1024;
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(TA_THREADS, 1)
+tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh, int slots_first_k, int slots_first_v, int chunk) {
+    typedef TreeMode<MODE> T;
+    constexpr int KEYS = T::KEYS, STAGES = T::STAGES, WORDS = KEYS / 32;
+    GLMB_PDL_PROLOGUE();  // before the TMEM allocation: a kernel still running may need the columns to finish
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], o_free[2], ml_full;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t fail;
+    __shared__ uint32_t page_bits[TA_NOTES][WORDS];  // keys of a block whose page exists
+    __shared__ unsigned long long broken[4];         // drafted values of a segment that are not finite
+    __shared__ float ml_s[128][2];
+    __shared__ int64_t run_s[3];
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const PagedArgs& c = a.cache;
+    const int kboxes = (c.dim + 63) / 64, vboxes = (c.vdim + 63) / 64;
+    unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* k_s = q_s + T::QTILES * T::BOXES * T::Q_BOX;
+    unsigned char* v_s = k_s + STAGES * T::BOXES * T::KV_BOX;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&ml_full, 4);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(o_free + i, 4);
+        for (int i = 0; i < STAGES; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
+        for (int i = 0; i < 4; ++i) broken[i] = 0;
+        fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 9) {  // this CTA's run: equal numbers of blocks, in the order of the sequences
+        const int64_t total = tree_blocks(a, sh, c.seqs, lane), share = (total + sh.ctas - 1) / sh.ctas;
+        const int64_t first = min(total, share * (int)blockIdx.x), count = min(share, total - first);
+        int64_t before = 0;
+        int seq = 0, found = -1;
+        for (; seq < c.seqs && found < 0; seq += 32) {
+            int64_t mine = 0;
+            if (seq + lane < c.seqs) {
+                const TreeSeq s = tree_seq(a, seq + lane, blockIdx.x == 0);
+                mine = (int64_t)s.blocks(KEYS) * sh.units(s.rows) * c.G;
+            }
+            int64_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t add = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += add;
+            }
+            const uint32_t who = __ballot_sync(0xffffffffu, mine > 0 && first < before + upto && first >= before + upto - mine);
+            if (who) {
+                found = seq + __ffs(who) - 1;
+                const int64_t rest = first - (before + __shfl_sync(0xffffffffu, upto - mine, __ffs(who) - 1));
+                if (lane == 0) run_s[1] = found, run_s[2] = rest;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (blockIdx.x == 0)
+            for (int b = seq + lane; b < c.seqs; b += 32) tree_seq(a, b, true);  // the report on those not looked at
+        if (lane == 0) run_s[0] = found < 0 ? 0 : count;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    const float sink2 = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY;
-    float top = sink2, total = 0.f, f[4];
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_s[w][0]);
-    for (int w = 0; w < 4; ++w) {
-        f[w] = ml_s[w][1] == 0.f ? 0.f : exp2f(ml_s[w][0] - top);
-        total += f[w] * ml_s[w][1];
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 256 and 384
+
+    TreeWalk walk{run_s[0], 0, 0, 0};
+    if (walk.left > 0) {
+        walk.b = (int)run_s[1];
+        const int of = tree_seq(a, walk.b, false).blocks(KEYS);
+        walk.at = (int)(run_s[2] / of), walk.block0 = (int)(run_s[2] % of);
     }
-    if (a.sink) total += exp2f(sink2 - top);
-    for (int d = threadIdx.x; d < c.vdim; d += 128) {
-        float sum = 0.f;
-        for (int w = 0; w < 4; ++w)
-            if (f[w] != 0.f) sum += f[w] * o_s[w][d];
-        a.out[(int64_t)row * a.out_row + (int64_t)h * a.out_head + d] = __float2bfloat16_rn(total == 0.f ? 0.f : sum / total);
+    // blocks of a segment that group t takes, and the n-th of them (counted from the segment's first)
+    auto group_blocks = [&](const TreeSegment& s, int t) {
+        if (MODE == TA_PAIR) return s.unit * 2 + t < sh.tiles(s.seq.rows) ? s.blocks : 0;
+        if (MODE == TA_SINGLE) return (s.blocks + 1 - t) >> 1;
+        return t == 0 ? s.blocks : 0;
+    };
+    auto nth = [&](int t, int n) { return MODE == TA_SINGLE ? 2 * n + t : n; };
+
+    TreeSegment s;
+    uint32_t gone = 0;  // blocks of the segments before this one
+    int segment = 0;
+    if (warp == 9) {
+        bool ok = true;
+        for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
+            if (segment > 0 && !mbar_wait_warp(&q_empty, (segment - 1) & 1)) { fail = 1; break; }
+            const int tiles = MODE == TA_PAIR ? min(2, sh.tiles(s.seq.rows) - s.unit * 2) : 1;
+            if (lane == 0) broken[segment & 3] = 0;
+            __syncwarp();
+            if (elect_one()) {
+                mbar_expect_tx(&q_full, tiles * kboxes * sh.heads * sh.tile_rows * 128);
+                for (int t = 0; t < tiles; ++t) {
+                    const int tile = s.unit * sh.in_unit + t;
+                    for (int x = 0; x < kboxes; ++x)
+                        ta_tma_3d(q_s + (t * kboxes + x) * T::Q_BOX, &map_q, &q_full, x * 64, s.g * sh.per + tile % sh.head_blocks * sh.heads,
+                                  s.seq.row0 + tile / sh.head_blocks * sh.tile_rows);
+                }
+            }
+            __syncwarp();
+            const int chunks = KEYS / chunk, last = s.seq.length + s.seq.drafts;  // slots from `last` on hold nothing
+            auto page_of = [&](int block) {  // lane i: the page of the i-th chunk, or one behind the last (read as zeros)
+                const int slot = (s.block0 + block) * KEYS + lane * chunk;
+                if (block >= s.blocks || lane >= chunks || slot >= last) return c.pages;
+                const int page = paged_page(c, s.b, slot);
+                if (page < 0) raise_status(a.status, GLMB_STATUS_BAD_INDEX);
+                return page < 0 ? c.pages : page;
+            };
+            int page = page_of(0);
+            for (int j = 0; j < s.blocks; ++j) {
+                const uint32_t n = gone + j, st = n % STAGES, lap = n / STAGES;
+                const int next_page = page_of(j + 1), slot = (s.block0 + j) * KEYS + lane * chunk, in_page = slot % c.page;
+                if (lap > 0 && !mbar_wait_warp(k_empty + st, (lap - 1) & 1)) { fail = 1; ok = false; break; }
+                const uint32_t there = __ballot_sync(0xffffffffu, page < c.pages);
+                if (lane < WORDS) {
+                    uint32_t bits = 0;
+                    for (int i = 0; i < 32; i += 8) bits |= there >> ((lane * 32 + i) / chunk) & 1u ? 0xffu << i : 0u;
+                    page_bits[n % TA_NOTES][lane] = bits;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(k_full + st, kboxes * T::KV_BOX);  // releases the notes too
+                __syncwarp();
+                if (lane < chunks)
+                    for (int x = 0; x < kboxes; ++x)
+                        ta_tma_4d(k_s + (st * kboxes + x) * T::KV_BOX + lane * chunk * 128, &map_k, k_full + st, x * 64, slots_first_k ? in_page : s.g, slots_first_k ? s.g : in_page, page);
+                __syncwarp();
+                if (lap > 0 && !mbar_wait_warp(v_empty + st, (lap - 1) & 1)) { fail = 1; ok = false; break; }
+                if (lane == 0) mbar_expect_tx(v_full + st, vboxes * T::KV_BOX);
+                __syncwarp();
+                if (lane < chunks)
+                    for (int x = 0; x < vboxes; ++x)
+                        ta_tma_4d(v_s + (st * vboxes + x) * T::KV_BOX + lane * chunk * 128, &map_v, v_full + st, x * 64, slots_first_v ? in_page : s.g, slots_first_v ? s.g : in_page, page);
+                __syncwarp();
+                page = next_page;
+            }
+        }
+    } else if (warp == 8) {
+        const uint32_t idesc_s = umma_idesc_bf16(128, KEYS), idesc_o = umma_idesc_bf16(128, c.vdim) | (1u << 16);  // bit 16: B is MN-major
+        uint32_t done[2] = {0, 0}, uses[2] = {0, 0};  // blocks and segments of a group so far
+        bool ok = true;
+        for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
+            const int count[2] = {group_blocks(s, 0), group_blocks(s, 1)}, most = max(count[0], count[1]);
+            if (!mbar_wait_warp(&q_full, segment & 1)) { fail = 1; break; }
+            for (int j = -1; j < most && ok; ++j) {
+#pragma unroll
+                for (int t = 0; t < T::GROUPS; ++t) {
+                    if (ok && j >= 0 && j < count[t]) {  // O_t += P_t V
+                        const uint32_t n = gone + nth(t, j), st = n % STAGES;
+                        ok = (j > 0 || uses[t] == 0 || mbar_wait_warp(o_free + t, (uses[t] - 1) & 1)) && mbar_wait_warp(p_full + t, done[t] & 1) &&
+                             mbar_wait_warp(v_full + st, (n / STAGES) & 1);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t v_addr = smem_u32(v_s + st * vboxes * T::KV_BOX);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int piece = 0; piece < T::PIECES; ++piece)
+#pragma unroll
+                                for (int k = 0; k < KEYS / 16; ++k)
+                                    umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + piece * (KEYS / 2) + k * 8, ta_desc_mn(v_addr + k * 2048, T::KV_BOX), idesc_o,
+                                                 (j > 0 || piece > 0 || k > 0) ? 1u : 0u);
+                            if (MODE != TA_PAIR || t == 1 || count[1] == 0) umma_commit(v_empty + st);  // the values may be replaced once they have been read
+                            if (j + 1 == count[t]) umma_commit(o_full + t);
+                        }
+                        __syncwarp();
+                        ++done[t];
+                        if (j + 1 == count[t]) ++uses[t];
+                    }
+                    if (ok && j + 1 < count[t]) {  // S_t = Q_t K^T
+                        const uint32_t n = gone + nth(t, j + 1), st = n % STAGES;
+                        ok = mbar_wait_warp(k_full + st, (n / STAGES) & 1);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t q_addr = smem_u32(q_s + (MODE == TA_PAIR ? t : 0) * kboxes * T::Q_BOX), k_addr = smem_u32(k_s + st * kboxes * T::KV_BOX);
+                        if (elect_one()) {
+                            for (int k = 0; k < c.dim / 16; ++k)
+                                umma_bf16(tmem + t * 128, umma_desc_sw128(q_addr + (k >> 2) * T::Q_BOX + (k & 3) * 32), umma_desc_sw128(k_addr + (k >> 2) * T::KV_BOX + (k & 3) * 32), idesc_s,
+                                          k > 0 ? 1u : 0u);
+                            umma_commit(s_full + t);
+                            if (MODE != TA_PAIR || t == 1 || count[1] == 0) umma_commit(k_empty + st);
+                            if (nth(t, j + 1) + 1 == s.blocks && (MODE != TA_PAIR || t == 1 || count[1] == 0)) umma_commit(&q_empty);  // the segment's last scores
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (!ok || __any_sync(0xffffffffu, fail)) { fail = 1; ok = false; }
+            }
+        }
+    } else {
+        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_addr = tmem + t * 128 + lanes;
+        const float scale2 = a.scale * TA_LOG2E;
+        const bool fixes = MODE != TA_PAIR || t == 0;  // of two tiles the first one's products come first
+        uint32_t seen = 0, used[2] = {0, 0}, joined = 0;  // blocks of this group, segments of each group, segments in which both had blocks
+        bool ok = true;
+        for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
+            const int count = group_blocks(s, t), other = MODE == TA_SINGLE ? group_blocks(s, 1 - t) : 0;
+            if (count == 0) {
+                if (other) ++used[1 - t];
+                continue;
+            }
+            const int tile = s.unit * sh.in_unit + (MODE == TA_PAIR ? t : 0), j0 = tile / sh.head_blocks * sh.tile_rows, h0 = tile % sh.head_blocks * sh.heads;
+            const int j = j0 + row / sh.heads, hh = h0 + row % sh.heads;
+            const bool live = row < sh.heads * sh.tile_rows && j < s.seq.rows && hh < sh.per, warp_live = __any_sync(0xffffffffu, live);
+            const uint64_t drafts = s.seq.drafts >= 64 ? ~0ull : (1ull << s.seq.drafts) - 1ull;
+            const uint64_t mask = live ? (uint64_t)a.masks[s.seq.row0 + j] & drafts : 0;
+            float m = -INFINITY, l = 0.f;
+            for (int n = 0; n < count; ++n) {
+                const int block = s.block0 + nth(t, n), base = block * KEYS;
+                const uint32_t number = gone + nth(t, n), st = number % STAGES;
+                if (!mbar_wait(s_full + t, seen & 1) || fail) { ok = false; break; }
+                ++seen;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t there = ~0u;
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) there &= page_bits[number % TA_NOTES][w];
+                const bool drafted = base + KEYS > s.seq.length;
+                if (warp_live) {
+                    uint32_t x[KEYS];
+#pragma unroll
+                    for (int i = 0; i < WORDS; ++i) ta_tmem_ld32_nowait(s_addr + i * 32, x + i * 32);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (drafted || there != ~0u) {
+#pragma unroll
+                        for (int w = 0; w < WORDS; ++w) {
+                            const uint32_t sees = ta_visible(base + w * 32 - s.seq.length, mask) & page_bits[number % TA_NOTES][w];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!(sees >> i & 1)) x[w * 32 + i] = 0xff800000u;  // -infinity
+                        }
+                    }
+                    float top[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+#pragma unroll
+                    for (int i = 4; i < KEYS; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    if (n == 0) {
+                        m = most;
+                    } else if (__any_sync(0xffffffffu, most > m + TA_SLACK)) {
+                        const float next = fmaxf(m, most), fix = next == -INFINITY ? 1.f : ta_exp2(m - next);
+                        m = next;
+                        l *= fix;
+                        for (int x0 = 0; x0 < c.vdim; x0 += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tmem + 256 + t * 128 + lanes + x0, o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                            ta_tmem_st16(tmem + 256 + t * 128 + lanes + x0, o);
+                        }
+                    }
+                    const float from = m == -INFINITY ? 0.f : m;
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WORDS; ++w) {
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float p = ta_exp2(fmaf(__uint_as_float(x[w * 32 + 2 * i]), scale2, -from)), r = ta_exp2(fmaf(__uint_as_float(x[w * 32 + 2 * i + 1]), scale2, -from));
+                            sum0 += p;
+                            sum1 += r;
+                            hi[i] = pack_bf16(p, r);
+                            if (T::PIECES == 2) lo[i] = pack_bf16(p - bf16_lo(hi[i]), r - bf16_hi(hi[i]));
+                        }
+                        ta_tmem_st16(s_addr + w * 16, hi);
+                        if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + w * 16, lo);
+                    }
+                    l += sum0 + sum1;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                if (drafted && fixes) {  // values that nobody, or not everybody, may multiply
+                    if (!mbar_wait(v_full + st, (number / STAGES) & 1)) { ok = false; break; }
+                    const int key = (KEYS / 4) * quarter + lane, draft = base + key - s.seq.length;
+                    if (lane < KEYS / 4 && draft >= 0) {
+                        unsigned char* at = v_s + st * vboxes * T::KV_BOX + key * 128;
+                        bool clear = draft >= s.seq.drafts;
+                        for (int x = 0; x < vboxes * 8 && !clear; ++x) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(at + (x >> 3) * T::KV_BOX + (((x & 7) ^ (key & 7)) << 4));
+                            for (uint32_t word : {u.x, u.y, u.z, u.w}) clear |= (word & 0x7f80u) == 0x7f80u || (word & 0x7f800000u) == 0x7f800000u;
+                        }
+                        if (clear) {
+                            for (int x = 0; x < vboxes * 8; ++x) *reinterpret_cast<uint4*>(at + (x >> 3) * T::KV_BOX + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            if (draft < s.seq.drafts) atomicOr(&broken[segment & 3], 1ull << draft);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t);
+            }
+            // the output of the segment: group 0 of a single tile takes what group 1 has along
+            if (MODE == TA_SINGLE && t == 1) {
+                if (ok && (used[1] == 0 || mbar_wait(o_free + 1, (used[1] - 1) & 1))) {
+                    ml_s[row][0] = m, ml_s[row][1] = l;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ml_full);
+                } else {
+                    ok = false;
+                }
+                ++used[0], ++used[1];
+                if (!ok) break;
+                continue;
+            }
+            const bool both = MODE == TA_SINGLE && other > 0;
+            if (ok) ok = mbar_wait(o_full + t, used[t] & 1) && !fail;
+            if (ok && both) ok = mbar_wait(o_full + 1, used[1] & 1) && mbar_wait(&ml_full, joined & 1) && !fail;
+            ++used[t];
+            if (both) ++used[1], ++joined;
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t lost = broken[segment & 3] & mask;
+            const bool whole = s.blocks == s.of;  // no other CTA has keys of this unit
+            if (warp_live) {
+                float f0 = 1.f, f1 = 0.f;
+                if (both) {
+                    const float m1 = ml_s[row][0], l1 = ml_s[row][1], next = fmaxf(m, m1);
+                    f0 = m == next ? 1.f : ta_exp2(m - next);
+                    f1 = m1 == next ? 1.f : ta_exp2(m1 - next);
+                    l = l * f0 + l1 * f1;
+                    m = isnan(m1) ? m1 : next;
+                }
+                const int head = s.g * sh.per + hh, out_row = s.seq.row0 + j;
+                float scale = 1.f;
+                if (whole) {
+                    if (a.sink && live && a.sink[head] != -INFINITY) {
+                        const float sink2 = a.sink[head] * TA_LOG2E, next = fmaxf(m, sink2), f = m == -INFINITY ? 0.f : ta_exp2(m - next);
+                        scale = f / (l * f + ta_exp2(sink2 - next));
+                    } else {
+                        scale = l == 0.f ? 0.f : 1.f / l;
+                    }
+                }
+                bf16* dst = a.out + (int64_t)out_row * a.out_row + (int64_t)head * a.out_head;
+                const int64_t slot = ((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x;
+                const int64_t part = (slot * sh.in_unit + (MODE == TA_PAIR ? t : 0)) * (sh.heads * sh.tile_rows) + row;
+                for (int x0 = 0; x0 < c.vdim; x0 += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tmem + 256 + t * 128 + lanes + x0, o);
+                    float y[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(o[i]);
+                    if (both) {
+                        tmem_ld16(tmem + 384 + lanes + x0, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = y[i] * f0 + __uint_as_float(o[i]) * f1;
+                    }
+                    if (!live) continue;
+                    for (uint64_t left = lost; left; left &= left - 1) {  // drafted values that were left out of the product
+                        const int drafted_slot = s.seq.length + __ffsll(left) - 1, page = paged_page(c, s.b, drafted_slot);
+                        const bf16* k = c.k + page * c.k_page + (drafted_slot % c.page) * c.k_slot + s.g * c.k_head;
+                        const bf16* v = c.v + page * c.v_page + (drafted_slot % c.page) * c.v_slot + s.g * c.v_head + x0;
+                        const bf16* q = a.q + (int64_t)out_row * a.q_row + (int64_t)head * a.q_head;
+                        float dot = 0.f;
+                        for (int d = 0; d < c.dim; ++d) dot = fmaf(to_f32(q[d]), to_f32(k[d]), dot);
+                        const float p = ta_exp2(fmaf(dot, scale2, -m));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = fmaf(p, to_f32(v[i]), y[i]);
+                    }
+                    if (whole) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = pack_bf16(y[2 * i] * scale, y[2 * i + 1] * scale);
+                        *reinterpret_cast<uint4*>(dst + x0) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(dst + x0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(a.part_o + part * c.vdim + x0 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                    }
+                }
+                if (live && !whole) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m, l);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(o_free + t);
+                if (both) mbar_arrive(o_free + 1);
+            }
+        }
+        if (!ok) {
+            fail = 1;
+            if (lane == 0) raise_status(a.status, GLMB_STATUS_WAIT_TIMEOUT);
+        }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 8) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// One CTA a row: joins the sums that several runs left of its heads, or clears the row where it belongs to no sequence.
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh) {
+    GLMB_PDL_PROLOGUE();
+    __shared__ int64_t before_s[2];
+    const PagedArgs& c = a.cache;
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int low = 0, high = c.seqs;  // the last sequence that begins at or before the row
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (a.starts[mid] <= row) low = mid;
+        else high = mid;
+    }
+    const int b = low;
+    const TreeSeq seq = tree_seq(a, b, false);
+    const int j = row - seq.row0;
+    if (j < 0 || j >= seq.rows) {
+        if (a.clear_rest)
+            for (int i = threadIdx.x; i < a.H * (c.vdim >> 3); i += 256) {
+                const int h = i / (c.vdim >> 3), d = i % (c.vdim >> 3) * 8;
+                *reinterpret_cast<uint4*>(a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head + d) = make_uint4(0, 0, 0, 0);
+            }
+        return;
+    }
+    if (warp < 2) {
+        const int64_t sum = tree_blocks(a, sh, warp == 0 ? c.seqs : b, lane);
+        if (lane == 0) before_s[warp] = sum;
+    }
+    __syncthreads();
+    const int64_t share = (before_s[0] + sh.ctas - 1) / sh.ctas;
+    const int blocks = seq.blocks(sh.keys), units = sh.units(seq.rows);
+    const int pieces = c.vdim >> 2;  // of four columns
+    for (int i = threadIdx.x; i < a.H * pieces; i += 256) {
+        const int h = i / pieces, d = i % pieces * 4, g = h / sh.per, hh = h % sh.per;
+        const int tile = j / sh.tile_rows * sh.head_blocks + hh / sh.heads, unit = tile / sh.in_unit;
+        const int64_t from = before_s[1] + ((int64_t)g * units + unit) * blocks;
+        const int first = (int)(from / share), last = (int)((from + blocks - 1) / share);  // CTAs with keys of the unit
+        if (first == last) continue;  // written already
+        const int64_t slot = ((int64_t)b * c.G + g) * sh.units_max + unit, in = j % sh.tile_rows * sh.heads + hh % sh.heads;
+        auto part = [&](int cta) { return ((slot + cta) * sh.in_unit + tile % sh.in_unit) * (sh.heads * sh.tile_rows) + in; };
+        float m = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int cta = first; cta <= last; ++cta) {
+            const int64_t p = part(cta);
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+            const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * c.vdim + d);
+            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing there
+            const float next = fmaxf(m, ml.x), f0 = m == next ? 1.f : ta_exp2(m - next), f1 = ml.x == next ? 1.f : ta_exp2(ml.x - next);
+            m = next;
+            l = l * f0 + ml.y * f1;
+            o[0] = o[0] * f0 + v.x * f1, o[1] = o[1] * f0 + v.y * f1, o[2] = o[2] * f0 + v.z * f1, o[3] = o[3] * f0 + v.w * f1;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------
+static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
+    TreeShape sh;
+    sh.per = a.H / a.cache.G;
+    sh.heads = sh.per < 128 ? sh.per : 128;
+    sh.head_blocks = ceil_div(sh.per, sh.heads);
+    sh.tile_rows = min(128 / sh.heads, a.max_rows);
+    const int tiles = ceil_div(a.max_rows, sh.tile_rows) * sh.head_blocks;
+    mode = a.cache.dim > 128 || a.cache.vdim > 128 ? TA_WIDE : tiles > 1 ? TA_PAIR : TA_SINGLE;
+    sh.in_unit = mode == TA_PAIR ? 2 : 1;
+    sh.keys = mode == TA_WIDE ? 64 : 128;
+    sh.ctas = 148;
+    sh.units_max = ceil_div(tiles, sh.in_unit);
+    return sh;
+}
+// Sums that all segments may leave: one for each unit and one more for each CTA.
+static int64_t tree_parts(const TreeAttentionArgs& a, const TreeShape& sh) {
+    return ((int64_t)a.cache.seqs * a.cache.G * sh.units_max + sh.ctas) * sh.in_unit * sh.heads * sh.tile_rows;
+}
+static int tree_refuses(const TreeAttentionArgs& a) {
+    const PagedArgs& c = a.cache;
+    return a.rows < 0 || c.G < 1 || a.H < 1 || a.H % c.G || c.dim < 16 || c.dim > 256 || c.dim % 16 || c.vdim < 16 || c.vdim > 256 || c.vdim % 16 || c.page < 8 || c.page % 8 ||
+           a.max_rows < 1 || a.max_rows > TA_MAX_DRAFTS || c.seqs < 0 || c.pages < 1 || !(a.scale > 0.f) || (int64_t)c.per_seq * c.page > 0x7fffff00;
+}
+
+static int tree_pool_map(CUtensorMap* map, const void* base, const PagedArgs& c, int width, int64_t page, int64_t slot, int64_t head, int rows, int& slots_first) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return 1;
+    slots_first = slot < head;  // the smaller stride first
+    const cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)(slots_first ? c.page : c.G), (cuuint64_t)(slots_first ? c.G : c.page), (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(slots_first ? slot : head) * 2, (cuuint64_t)(slots_first ? head : slot) * 2, (cuuint64_t)page * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(slots_first ? rows : 1), (cuuint32_t)(slots_first ? 1 : rows), 1}, elem[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
+}
+static int tree_query_map(CUtensorMap* map, const TreeAttentionArgs& a, const TreeShape& sh) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return 1;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.cache.dim, (cuuint64_t)a.H, (cuuint64_t)a.rows}, strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_row * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)sh.heads, (cuuint32_t)sh.tile_rows}, elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
+}
+
+template <int MODE>
+static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStream_t stream) {
+    typedef TreeMode<MODE> T;
+    int chunk = 8;  // slots that lie in one page wherever a block begins
+    while (chunk < T::KEYS && a.cache.page % (2 * chunk) == 0) chunk *= 2;
+    const PagedArgs& c = a.cache;
+    CUtensorMap map_q, map_k, map_v;
+    int first_k, first_v;
+    if (tree_query_map(&map_q, a, sh) || tree_pool_map(&map_k, c.k, c, c.dim, c.k_page, c.k_slot, c.k_head, chunk, first_k) ||
+        tree_pool_map(&map_v, c.v, c, c.vdim, c.v_page, c.v_slot, c.v_head, chunk, first_v))
+        return 3;
+    static DeviceOnce once;
+    const int dev = once.pending();
+    if (dev != DeviceOnce::SET) {
+        const cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        if (e != cudaSuccess) return (int)e;
+        once.mark(dev);
+    }
+    GLMB_LAUNCH(tree_attention_kernel<MODE>, sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    GLMB_LAUNCH(tree_merge_kernel, a.rows, 256, 0, stream, a, sh);
+    return (int)cudaGetLastError();
 }
 
 GLMB_API size_t glmb_tree_attention_args_sizeof() { return sizeof(TreeAttentionArgs); }
 
+// Sums that a call needs room for: each vdim + 2 floats; -1: the call is refused.
+GLMB_API int64_t glmb_tree_attention_parts(const TreeAttentionArgs* args) {
+    if (tree_refuses(*args)) return -1;
+    int mode;
+    const TreeShape sh = tree_shape(*args, mode);
+    return tree_parts(*args, sh);
+}
+
 GLMB_API int glmb_tree_attention(const TreeAttentionArgs* args, cudaStream_t stream) {
     const TreeAttentionArgs a = *args;
-    const PagedArgs& c = a.cache;
-    if (a.rows < 0 || c.G < 1 || a.H < 1 || a.H % c.G || c.dim < 16 || c.dim > 256 || c.dim % 16 || c.vdim < 16 || c.vdim > 256 || c.vdim % 16 || c.page < 1 ||
-        a.max_rows < 1 || a.max_rows > TA_MAX_DRAFTS || c.seqs < 0 || c.seqs > 65535 || (int64_t)c.per_seq * c.page > 0x7fffff00)
-        return 1;
-    if (c.seqs == 0 || a.rows == 0) return 0;
-    GLMB_LAUNCH(tree_attention_kernel, dim3(a.H, a.max_rows, c.seqs), 128, 0, stream, a);
-    return (int)cudaGetLastError();
+    if (tree_refuses(a)) return 1;
+    if (a.cache.seqs == 0 || a.rows == 0) return 0;
+    int mode;
+    const TreeShape sh = tree_shape(a, mode);
+    if (a.parts < tree_parts(a, sh) || !a.part_o || !a.part_ml) return 1;
+    return mode == TA_PAIR ? tree_launch<TA_PAIR>(a, sh, stream) : mode == TA_SINGLE ? tree_launch<TA_SINGLE>(a, sh, stream) : tree_launch<TA_WIDE>(a, sh, stream);
 }

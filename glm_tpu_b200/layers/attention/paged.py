@@ -11,6 +11,7 @@ int32 tensor of one element on the same GPU) as a bad index, the row stores noth
 
 from __future__ import annotations
 
+import math
 from collections.abc import Sequence
 from dataclasses import dataclass
 
@@ -27,7 +28,7 @@ class PagedKV:
     """A pool of pages and the table that says which of them hold a sequence's slots: slot ``s`` of sequence ``b`` is row ``s % page`` of page
     ``table[b, s // page]``.  Entries behind a sequence's last page may hold anything."""
 
-    k: torch.Tensor  # [pages, page, kv_heads, dim] bf16, heads' channels contiguous
+    k: torch.Tensor  # [pages, page, kv_heads, dim] bf16, a head's channels contiguous; page: a multiple of 8
     v: torch.Tensor  # [pages, page, kv_heads, vdim]
     table: torch.Tensor  # [sequences, pages of a sequence] int32
 
@@ -46,8 +47,8 @@ def ancestor_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _check_cache(cache: PagedKV, device: torch.device) -> None:
     k, v, table = cache.k, cache.v, cache.table
-    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.shape[1] or not k.shape[2]:
-        raise ValueError("pools are [pages, page, kv_heads, dim] and [pages, page, kv_heads, vdim] in bf16")
+    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.numel() or not v.numel() or k.shape[1] % 8:
+        raise ValueError("pools are [pages, page, kv_heads, dim] and [pages, page, kv_heads, vdim] in bf16, with a multiple of 8 slots a page")
     if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1) or table.shape[1] * k.shape[1] > MAX_SLOTS:
         raise ValueError("the table is [sequences, pages of a sequence] in int32, of up to 2^30 slots a sequence")
     if k.device != device or v.device != device or table.device != device:
@@ -121,6 +122,8 @@ def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, length
     _check_index("masks", masks, rows, torch.int64, q.device)
     if not 1 <= max_rows <= MAX_DRAFTS:
         raise ValueError(f"between 1 and {MAX_DRAFTS} rows a sequence")
+    if not 0.0 < scale < math.inf:
+        raise ValueError("the scale is positive")
     if sink is not None:
         _check_index("sink", sink, heads, torch.float32, q.device)
     if out is not None and (out.shape != (rows, heads, vdim) or out.dtype != torch.bfloat16 or out.device != q.device):

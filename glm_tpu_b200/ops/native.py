@@ -176,7 +176,7 @@ class TreeAttentionArgs(C.Structure):
         ("cache", PagedArgs),
         ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64),
         ("starts", C.c_void_p), ("lengths", C.c_void_p), ("masks", C.c_void_p), ("sink", C.c_void_p),
-        ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("splits", C.c_int),
+        ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("parts", C.c_int64),
         ("rows", C.c_int), ("H", C.c_int), ("max_rows", C.c_int), ("scale", C.c_float), ("clear_rest", C.c_int),
         ("status", C.c_void_p),
     ]
@@ -216,6 +216,8 @@ def lib() -> C.CDLL:
         _lib.glmb_peer_status_ptr.restype = C.c_void_p
         if hasattr(_lib, "glmb_indexer_rows_scratch_bytes"):  # a component library holds one family's kernels only
             _lib.glmb_indexer_rows_scratch_bytes.restype = C.c_int64
+        if hasattr(_lib, "glmb_tree_attention_parts"):
+            _lib.glmb_tree_attention_parts.restype = C.c_int64
         for entry, struct in _STRUCTS:
             if not hasattr(_lib, entry):  # a component library holds one family's kernels only
                 continue
@@ -928,8 +930,13 @@ def tree_attention(q, k, v, table, starts, lengths, masks, scale, max_rows, sink
     """Attention of drafted rows over a paged cache and their ancestors (``layers.attention.paged.tree_attention``)."""
     rows, H, _ = q.shape
     a = TreeAttentionArgs(_paged(k, v, table), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), starts.data_ptr(), lengths.data_ptr(),
-                          masks.data_ptr(), None if sink is None else sink.data_ptr(), None, None, 1, rows, H, max_rows, scale, int(clear_rest),
+                          masks.data_ptr(), None if sink is None else sink.data_ptr(), None, None, 0, rows, H, max_rows, scale, int(clear_rest),
                           None if status is None else status.data_ptr())
+    lib()
+    parts = _lib.glmb_tree_attention_parts(C.byref(a))  # not a launch: past the wrapper that times launches
+    vdim = v.shape[3]
+    room = torch.empty(max(parts, 0) * (vdim + 2), dtype=torch.float32, device=q.device)  # sums of keys that several CTAs share
+    a.part_o, a.part_ml, a.parts = room.data_ptr(), room.data_ptr() + 4 * parts * vdim, parts
     _check(lib().glmb_tree_attention(C.byref(a), _stream()), "tree_attention")
 
 

@@ -58,8 +58,8 @@ def assert_append(c, pairs=False):
 @pytest.mark.gpu
 @pytest.mark.parametrize("pairs", [False, True])
 @pytest.mark.parametrize("rows, H, G, dim, vdim, page, rot, norm", [
-    (1, 1, 1, 16, 16, 1, 16, True), (1, 16, 4, 128, 128, 64, 64, True), (7, 8, 2, 64, 32, 5, 0, True), (33, 32, 8, 128, 128, 64, 128, True), (5, 4, 4, 80, 64, 16, 6, True),
-    (65, 6, 3, 192, 256, 24, 192, False), (300, 3, 1, 256, 16, 7, 34, True), (2, 64, 8, 96, 96, 128, 48, False), (129, 12, 2, 48, 48, 33, 46, True)])
+    (1, 1, 1, 16, 16, 8, 16, True), (1, 16, 4, 128, 128, 64, 64, True), (7, 8, 2, 64, 32, 40, 0, True), (33, 32, 8, 128, 128, 64, 128, True), (5, 4, 4, 80, 64, 16, 6, True),
+    (65, 6, 3, 192, 256, 24, 192, False), (300, 3, 1, 256, 16, 8, 34, True), (2, 64, 8, 96, 96, 128, 48, False), (129, 12, 2, 48, 48, 56, 46, True)])
 def test_append(native_lib, rows, H, G, dim, vdim, page, rot, norm, pairs):
     assert_append(append_case(rows, H, G, dim, vdim, page, rot=rot, norm=norm), pairs)
 
@@ -114,8 +114,8 @@ def test_append_of_zero_rows_and_of_zeros(native_lib):
 
 # ------------------------------------------------------------------------------------------------ attention
 SHAPES = [  # lengths, drafted tokens, heads, kv heads, dim, vdim, page
-    ([0], [1], 1, 1, 16, 16, 1), ([1], [1], 4, 2, 64, 64, 16), ([777], [1], 16, 4, 128, 128, 64), ([63, 64, 65], [1, 1, 1], 8, 8, 128, 128, 64), ([0, 5, 300], [3, 7, 2], 8, 2, 64, 128, 16),
-    ([100], [64], 8, 1, 128, 64, 24), ([129, 0, 1000, 17], [16, 1, 33, 8], 32, 8, 128, 128, 64), ([500], [5], 12, 2, 80, 80, 48), ([255], [9], 6, 3, 192, 192, 7), ([321, 4], [11, 64], 64, 8, 128, 128, 128),
+    ([0], [1], 1, 1, 16, 16, 8), ([1], [1], 4, 2, 64, 64, 16), ([777], [1], 16, 4, 128, 128, 64), ([63, 64, 65], [1, 1, 1], 8, 8, 128, 128, 64), ([0, 5, 300], [3, 7, 2], 8, 2, 64, 128, 16),
+    ([100], [64], 8, 1, 128, 64, 24), ([129, 0, 1000, 17], [16, 1, 33, 8], 32, 8, 128, 128, 64), ([500], [5], 12, 2, 80, 80, 48), ([255], [9], 6, 3, 192, 192, 8), ([321, 4], [11, 64], 64, 8, 128, 128, 128),
     ([2047], [2], 8, 8, 256, 256, 32), ([60], [64], 20, 1, 96, 48, 64), ([3000, 1], [4, 4], 7, 7, 32, 16, 16)]
 
 
