@@ -24,17 +24,12 @@ struct LogitSums {
     float m, s, t;
     __device__ __forceinline__ void clear() { m = -INFINITY, s = 0.f, t = 0.f; }
     __device__ __forceinline__ void join(const LogitSums& o) {
-        if (o.m == -INFINITY) return;
-        if (m == -INFINITY) {
-            *this = o;
-            return;
-        }
         const bool mine = m >= o.m;
-        const LogitSums high = mine ? *this : o, low = mine ? o : *this;
-        const float d = low.m - high.m, f = lp_exp2(d * LP_LOG2E), sum = 1.f + low.s;
-        m = high.m;
-        s = fmaf(sum, f, high.s);
-        t = high.t + (f > 0.f ? fmaf(sum, d, low.t) * f : 0.f);  // d may be minus infinity
+        const float hm = mine ? m : o.m, hs = mine ? s : o.s, ht = mine ? t : o.t, lm = mine ? o.m : m, ls = mine ? o.s : s, lt = mine ? o.t : t;
+        const float d = lm - hm, f = lm == -INFINITY ? 0.f : lp_exp2(d * LP_LOG2E), sum = 1.f + ls;
+        m = hm;
+        s = fmaf(sum, f, hs);
+        t = ht + (f > 0.f ? fmaf(sum, d, lt) * f : 0.f);  // d may be minus infinity
     }
     __device__ __forceinline__ void join_lanes(int lanes) {  // of a warp's first `lanes` (a power of two): the same result on each
         for (int o = lanes >> 1; o > 0; o >>= 1) {

@@ -151,6 +151,15 @@ class TokenLogprobsArgs(C.Structure):
     ]
 
 
+class HeadLogprobsArgs(C.Structure):
+    _fields_ = [
+        ("hidden", C.c_void_p), ("hidden_stride", C.c_int64), ("head", C.c_void_p), ("head_stride", C.c_int64),
+        ("scores", TokenScores),
+        ("part", C.c_void_p), ("given", C.c_void_p), ("parts", C.c_int64),
+        ("rows", C.c_int), ("vocab", C.c_int), ("width", C.c_int),
+    ]
+
+
 class PagedArgs(C.Structure):
     _fields_ = [
         ("k", C.c_void_p), ("k_page", C.c_int64), ("k_slot", C.c_int64), ("k_head", C.c_int64),
@@ -185,6 +194,7 @@ class TreeAttentionArgs(C.Structure):
 # argument structures and the entry point that gives their size in the library
 _STRUCTS = (("glmb_qkv_conv_args_sizeof", QkvConvArgs), ("glmb_chunk_attn_args_sizeof", ChunkAttnArgs), ("glmb_latent_args_sizeof", LatentArgs),
             ("glmb_delta_args_sizeof", DeltaArgs), ("glmb_token_logprobs_args_sizeof", TokenLogprobsArgs),
+            ("glmb_head_logprobs_args_sizeof", HeadLogprobsArgs),
             ("glmb_paged_append_args_sizeof", PagedAppendArgs), ("glmb_tree_attention_args_sizeof", TreeAttentionArgs))
 
 _lib = None
@@ -216,8 +226,9 @@ def lib() -> C.CDLL:
         _lib.glmb_peer_status_ptr.restype = C.c_void_p
         if hasattr(_lib, "glmb_indexer_rows_scratch_bytes"):  # a component library holds one family's kernels only
             _lib.glmb_indexer_rows_scratch_bytes.restype = C.c_int64
-        if hasattr(_lib, "glmb_tree_attention_parts"):
-            _lib.glmb_tree_attention_parts.restype = C.c_int64
+        for entry in ("glmb_tree_attention_parts", "glmb_head_logprobs_parts"):
+            if hasattr(_lib, entry):
+                getattr(_lib, entry).restype = C.c_int64
         for entry, struct in _STRUCTS:
             if not hasattr(_lib, entry):  # a component library holds one family's kernels only
                 continue
@@ -890,22 +901,30 @@ def token_logprobs(logits, tokens, sums, top_ids=None, top_logprobs=None, *, sta
     _check(lib().glmb_token_logprobs(C.byref(a), _stream()), "token_logprobs")
 
 
-HEAD_SLAB = 1 << 26  # logits of a slab of rows
+HEAD_SLAB = 1 << 26  # fp32: logits of a slab of rows
 
 
 def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
-    """``token_logprobs`` of ``hidden @ head[:vocab].T``, some rows at a time."""
-    rows = hidden.shape[0]
-    step = max(1, min(rows, HEAD_SLAB // head.shape[0]))
-    padded = -(-head.shape[0] // 8) * 8
-    logits = torch.empty((step, padded), dtype=torch.float32, device=hidden.device)
-    for r in range(0, rows, step):
+    """``token_logprobs`` (without alternatives) of ``hidden @ head[:vocab].T``.  bf16: one to eight rows stream the table once and leave their logits in L2; more
+    rows form them on tcgen05 and keep sums only.  fp32 (plain FMA): some rows at a time."""
+    rows, width = hidden.shape
+    if hidden.dtype == torch.bfloat16 and rows > MAX_ROWS:
+        lib()
+        parts = _lib.glmb_head_logprobs_parts(rows, vocab)  # not a launch: past the wrapper that times launches
+        room = torch.empty((4 * parts + 1) * rows, dtype=torch.float32, device=hidden.device)
+        part = room.data_ptr()
+        a = HeadLogprobsArgs(hidden.data_ptr(), hidden.stride(0), head.data_ptr(), head.stride(0), _scores(tokens, sums, status), part, part + 16 * parts * rows, parts,
+                             rows, vocab, width)
+        _check(lib().glmb_head_logprobs(C.byref(a), _stream()), "head_logprobs")
+        return
+    step = rows if hidden.dtype == torch.bfloat16 else max(1, min(rows, HEAD_SLAB // vocab))
+    logits = torch.empty((step, -(-vocab // 8) * 8), dtype=torch.float32, device=hidden.device)
+    for r in range(0, rows, max(step, 1)):
         n = min(step, rows - r)
         if hidden.dtype == torch.float32:
-            gemm_f32(hidden[r : r + n], head, logits[:n])
+            gemm_f32(hidden[r : r + n], head[:vocab], logits[:n])
         else:
-            for i in range(0, n, MAX_ROWS):
-                skinny_bf16(hidden[r + i : r + min(n, i + MAX_ROWS)], head, logits[i:n], SK_OUT_F32)
+            skinny_bf16(hidden, head, logits, SK_OUT_F32, N=vocab)
         token_logprobs(logits[:n, :vocab], tokens[r : r + n], sums[:, r : r + n], status=status)
 
 
