@@ -17,6 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
+from glm_tpu_b200.ops import native
 from glm_tpu_b200.oracle import scoring
 
 MAX_DRAFTS = 64
@@ -45,23 +46,31 @@ def ancestor_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
     return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64), torch.tensor(depths, dtype=torch.int32)
 
 
-def _check_cache(cache: PagedKV, device: torch.device) -> None:
+def _checked(cache: PagedKV, device: int) -> native.PagedArgs:
+    """The cache as the kernels take it; ``device``: where the rows lie (-1: CPU)."""
     k, v, table = cache.k, cache.v, cache.table
-    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or not k.numel() or not v.numel() or k.shape[1] % 8:
+    if k.dim() != 4 or v.dim() != 4 or table.dim() != 2:
+        raise ValueError("pools have four axes, the table two")
+    pages, page, G, dim = k.shape
+    vdim, (seqs, per_seq) = v.shape[3], table.shape
+    k_page, k_slot, k_head, k_last = k.stride()
+    v_page, v_slot, v_head, v_last = v.stride()
+    if v.shape[:3] != k.shape[:3] or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or not pages or not page or page % 8 or not G:
         raise ValueError("pools are [pages, page, kv_heads, dim] and [pages, page, kv_heads, vdim] in bf16, with a multiple of 8 slots a page")
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1) or table.shape[1] * k.shape[1] > MAX_SLOTS:
+    if table.dtype is not torch.int32 or (per_seq > 1 and table.stride(1) != 1) or per_seq * page > MAX_SLOTS:
         raise ValueError("the table is [sequences, pages of a sequence] in int32, of up to 2^30 slots a sequence")
-    if k.device != device or v.device != device or table.device != device:
+    if k.get_device() != device or v.get_device() != device or table.get_device() != device:
         raise ValueError("rows, pools and table lie on one device")
-    dim, vdim = k.shape[3], v.shape[3]
     if not 16 <= dim <= 256 or not 16 <= vdim <= 256 or dim % 16 or vdim % 16:
         raise ValueError("heads are 16 to 256 channels wide, in multiples of 16")
-    if k.is_cuda and (k.stride(3) != 1 or v.stride(3) != 1 or any(s % 8 for s in (*k.stride()[:3], *v.stride()[:3])) or (k.data_ptr() | v.data_ptr()) % 16):
+    k_at, v_at = k.data_ptr(), v.data_ptr()
+    if device >= 0 and (k_last != 1 or v_last != 1 or (k_page | k_slot | k_head | v_page | v_slot | v_head) % 8 or (k_at | v_at) % 16):
         raise ValueError("the channels of a head are contiguous and every head of the pools 16-byte aligned")
+    return native.PagedArgs(k_at, k_page, k_slot, k_head, v_at, v_page, v_slot, v_head, table.data_ptr(), table.stride(0), seqs, per_seq, pages, page, G, dim, vdim)
 
 
-def _check_index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> None:
-    if t.shape != (n,) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+def _check_index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: int) -> None:
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name}: {n} contiguous elements of {str(dtype)[6:]} on the device of the rows")
 
 
@@ -73,32 +82,33 @@ def append(qkv: torch.Tensor, cache: PagedKV, positions: torch.Tensor | None, se
     ``rot``: fp32 ``[positions, n, 2]`` (cos, sin) for the leading ``2 n`` channels of q and k, as halves ``(d, d + n)`` or, with ``pairs``, as neighbours
     ``(2j, 2j + 1)``; ``q_norm`` / ``k_norm``: bf16 ``[dim]``, RMS norm of every head before the rotation.  A negative slot stores nothing.  Rows of one call name different
     slots.  ``want_q=False``: keys and values only (returns ``None``)."""
-    _check_cache(cache, qkv.device)
-    G, dim, vdim = cache.k.shape[2], cache.k.shape[3], cache.v.shape[3]
-    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or heads < 1 or qkv.shape[1] != heads * dim + G * (dim + vdim):
+    device = qkv.get_device()
+    args = _checked(cache, device)
+    dim = args.dim
+    if qkv.dim() != 2 or qkv.dtype is not torch.bfloat16 or heads < 1 or qkv.shape[1] != heads * dim + args.G * (dim + args.vdim):
         raise ValueError("qkv is [rows, heads * dim + kv_heads * (dim + vdim)] in bf16")
     rows = qkv.shape[0]
-    _check_index("seqs", seqs, rows, torch.int32, qkv.device)
-    _check_index("slots", slots, rows, torch.int32, qkv.device)
+    _check_index("seqs", seqs, rows, torch.int32, device)
+    _check_index("slots", slots, rows, torch.int32, device)
     if rot is not None:
         if positions is None:
             raise ValueError("a rotation needs positions")
-        _check_index("positions", positions, rows, torch.int32, qkv.device)
-        if rot.dim() != 3 or rot.shape[2] != 2 or 2 * rot.shape[1] > dim or not rot.shape[1] or rot.dtype != torch.float32 or not rot.is_contiguous() or rot.device != qkv.device:
+        _check_index("positions", positions, rows, torch.int32, device)
+        if rot.dim() != 3 or rot.shape[2] != 2 or not 0 < 2 * rot.shape[1] <= dim or rot.dtype is not torch.float32 or not rot.is_contiguous() or rot.get_device() != device:
             raise ValueError("rot is [positions, n, 2] in fp32, contiguous, with 2 n channels at most as many as a head has")
+    if status is not None:
+        _check_index("status", status, 1, torch.int32, device)
     for weight in (q_norm, k_norm):
         if weight is not None:
-            _check_index("norm", weight, dim, torch.bfloat16, qkv.device)
-    if not qkv.is_cuda:
+            _check_index("norm", weight, dim, torch.bfloat16, device)
+    if device < 0:
         q = scoring.append(qkv, cache.k, cache.v, cache.table, positions, seqs, slots, heads=heads, q_norm=q_norm, k_norm=k_norm, eps=eps, rot=rot, pairs=pairs)
         return q if want_q else None
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         raise ValueError("rows of qkv are contiguous and 16-byte aligned")
-    from glm_tpu_b200.ops import native
-
-    with torch.cuda.device(qkv.device):
-        q = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device=qkv.device) if want_q else None
-        native.paged_append(qkv, cache.k, cache.v, cache.table, positions, seqs, slots, q, heads, rot, pairs, q_norm, k_norm, eps, status=status)
+    with native.on_device(qkv):
+        q = qkv.new_empty((rows, heads, dim)) if want_q else None
+        native.paged_append(qkv, args, positions, seqs, slots, q, heads, rot, pairs, q_norm, k_norm, eps, status=status)
     return q
 
 
@@ -110,35 +120,37 @@ def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, length
     those, one per row in order.  ``masks`` (int64): bit ``t`` lets a row see its sequence's drafted slot ``t``; bits of rows that the sequence does
     not have mean nothing.  ``max_rows`` (at most 64): rows of the largest sequence.  ``sink``: fp32 ``[heads]``, a score that takes weight and gives no value.  A row
     that sees nothing, without a sink, is zeros.  Rows that belong to no sequence stay as they are in ``out``, or are zeros where it is made here."""
-    _check_cache(cache, q.device)
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != cache.k.shape[3] or not q.shape[1] or q.shape[1] % cache.k.shape[2]:
+    device = q.get_device()
+    args = _checked(cache, device)
+    seqs, vdim = args.seqs, args.vdim
+    if q.dim() != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != args.dim or not q.shape[1] or q.shape[1] % args.G:
         raise ValueError("q is [rows, heads, dim] in bf16, with a multiple of the cache's heads")
     rows, heads, _ = q.shape
-    seqs, vdim = cache.table.shape[0], cache.v.shape[3]
     if seqs > 65535:
         raise ValueError("at most 65,535 sequences")
-    _check_index("starts", starts, seqs + 1, torch.int32, q.device)
-    _check_index("lengths", lengths, seqs, torch.int32, q.device)
-    _check_index("masks", masks, rows, torch.int64, q.device)
+    _check_index("starts", starts, seqs + 1, torch.int32, device)
+    _check_index("lengths", lengths, seqs, torch.int32, device)
+    _check_index("masks", masks, rows, torch.int64, device)
     if not 1 <= max_rows <= MAX_DRAFTS:
         raise ValueError(f"between 1 and {MAX_DRAFTS} rows a sequence")
     if not 0.0 < scale < math.inf:
         raise ValueError("the scale is positive")
+    if status is not None:
+        _check_index("status", status, 1, torch.int32, device)
     if sink is not None:
-        _check_index("sink", sink, heads, torch.float32, q.device)
-    if out is not None and (out.shape != (rows, heads, vdim) or out.dtype != torch.bfloat16 or out.device != q.device):
+        _check_index("sink", sink, heads, torch.float32, device)
+    if out is not None and (out.shape != (rows, heads, vdim) or out.dtype is not torch.bfloat16 or out.get_device() != device):
         raise ValueError("out is [rows, heads, vdim] in bf16 on the device of q")
-    if not q.is_cuda:
+    if device < 0:
         out = torch.zeros((rows, heads, vdim), dtype=torch.bfloat16) if out is None else out
         return scoring.tree_attention(q, cache.k, cache.v, cache.table, starts, lengths, masks, scale, max_rows, sink, out)
-    for t in (q, out):
-        if t is not None and (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+    for t in (q,) if out is None else (q, out):
+        row, head, last = t.stride()
+        if last != 1 or (row | head) % 8 or t.data_ptr() % 16:
             raise ValueError("the channels of a head are contiguous and every head of q and out 16-byte aligned")
-    from glm_tpu_b200.ops import native
-
-    with torch.cuda.device(q.device):
+    with native.on_device(q):
         made = out is None
         if made:
-            out = (torch.empty if seqs else torch.zeros)((rows, heads, vdim), dtype=torch.bfloat16, device=q.device)
-        native.tree_attention(q, cache.k, cache.v, cache.table, starts, lengths, masks, scale, max_rows, sink, out, clear_rest=made, status=status)
+            out = (q.new_empty if seqs else q.new_zeros)((rows, heads, vdim))
+        native.tree_attention(q, args, starts, lengths, masks, scale, max_rows, sink, out, clear_rest=made, status=status)
     return out

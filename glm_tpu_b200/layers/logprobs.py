@@ -13,16 +13,19 @@ from __future__ import annotations
 import torch
 
 from glm_tpu_b200.layers.contracts import TokenLogprobs
+from glm_tpu_b200.ops import native
 from glm_tpu_b200.oracle import scoring
 
 MAX_TOP = 32
 
 
-def _check_tokens(tokens: torch.Tensor, rows: int, device: torch.device) -> None:
+def _check_tokens(tokens: torch.Tensor, rows: int, device: int, status: torch.Tensor | None) -> None:
     if tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"tokens are int32 or int64, one for each of the {rows} rows")
-    if tokens.device != device:
+    if tokens.get_device() != device:
         raise ValueError("tokens and rows lie on one device")
+    if status is not None and (status.numel() != 1 or status.dtype is not torch.int32 or status.get_device() != device):
+        raise ValueError("the status is one element of int32 on the device of the rows")
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, status: torch.Tensor | None = None) -> TokenLogprobs:
@@ -30,19 +33,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not logits.shape[1]:
         raise ValueError("logits are [rows, vocab] in bf16 or fp32")
     rows, vocab = logits.shape
-    _check_tokens(tokens, rows, logits.device)
+    _check_tokens(tokens, rows, logits.get_device(), status)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"between 0 and {min(MAX_TOP, vocab)} alternatives")
     if not logits.is_cuda:
         return scoring.token_logprobs(logits, tokens, top)
     if logits.stride(1) != 1 and vocab > 1:
         raise ValueError("logits are contiguous along a row")
-    from glm_tpu_b200.ops import native
-
-    with torch.cuda.device(logits.device):
-        sums = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device) if top else None
-        alternatives = torch.empty((rows, top), dtype=torch.float32, device=logits.device) if top else None
+    with native.on_device(logits):
+        sums = logits.new_empty((3, rows), dtype=torch.float32)
+        ids = logits.new_empty((rows, top), dtype=torch.int32) if top else None
+        alternatives = logits.new_empty((rows, top), dtype=torch.float32) if top else None
         native.token_logprobs(logits, tokens.contiguous(), sums, ids, alternatives, status=status)
     return TokenLogprobs(*sums.unbind(0), ids, alternatives)
 
@@ -56,16 +57,14 @@ def head_logprobs(hidden: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor
     vocab = head.shape[0] if vocab is None else int(vocab)
     if head.shape[1] != width or width < 1 or not 0 < vocab <= head.shape[0]:
         raise ValueError("the table has a row as wide as the hidden states for every token of the vocabulary")
-    _check_tokens(tokens, rows, hidden.device)
-    if head.device != hidden.device:
+    _check_tokens(tokens, rows, hidden.get_device(), status)
+    if head.get_device() != hidden.get_device():
         raise ValueError("hidden states and table lie on one device")
     if not hidden.is_cuda:
         return scoring.head_logprobs(hidden, head[:vocab], tokens)
     if width % 8 or hidden.stride(1) != 1 or head.stride(1) != 1 or hidden.stride(0) % 8 or head.stride(0) % 8 or (hidden.data_ptr() | head.data_ptr()) % 16:
         raise ValueError("rows of hidden states and table are contiguous, 16-byte aligned and a multiple of 8 wide")
-    from glm_tpu_b200.ops import native
-
-    with torch.cuda.device(hidden.device):
-        sums = torch.empty((3, rows), dtype=torch.float32, device=hidden.device)
+    with native.on_device(hidden):
+        sums = hidden.new_empty((3, rows), dtype=torch.float32)
         native.head_logprobs(hidden, head, vocab, tokens.contiguous(), sums, status=status)
     return TokenLogprobs(*sums.unbind(0), None, None)

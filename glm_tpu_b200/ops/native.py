@@ -348,6 +348,24 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_here = _Here()
+
+
+def on_device(t):
+    """A context in which the device of ``t`` is the current one; where it is already, entering it costs nothing."""
+    if _raw_device is not None and t.get_device() == _raw_device():
+        return _here
+    return torch.cuda.device(t.device)
+
+
 def _check(code: int, what: str) -> None:
     if code != 0:
         raise RuntimeError(f"{what} failed with code {code}")
@@ -929,34 +947,33 @@ def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
 
 
 # ----------------------------------------------------------------------------- drafted tokens over a paged cache
-def _paged(k, v, table) -> PagedArgs:
-    pages, page, G, dim = k.shape
-    ks, vs = k.stride(), v.stride()
-    return PagedArgs(k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], pages, page,
-                     G, dim, v.shape[3])
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def paged_append(qkv, k, v, table, positions, seqs, slots, q, heads, rot=None, pairs=False, q_norm=None, k_norm=None, eps=1e-6, *, status=None):
+def paged_append(qkv, cache: PagedArgs, positions, seqs, slots, q, heads, rot=None, pairs=False, q_norm=None, k_norm=None, eps=1e-6, *, status=None):
     """Norm and rotation of the heads of a fused projection; keys and values into the pages of their slots (``layers.attention.paged.append``)."""
-    a = PagedAppendArgs(_paged(k, v, table), qkv.data_ptr(), qkv.stride(0), None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
-                        None if rot is None else rot.data_ptr(), 0 if rot is None else 2 * rot.shape[1], 0 if rot is None else rot.shape[0], int(pairs),
-                        None if positions is None else positions.data_ptr(), seqs.data_ptr(), slots.data_ptr(), None if q is None else q.data_ptr(),
-                        heads * k.shape[3], qkv.shape[0], heads, eps, None if status is None else status.data_ptr())
+    half, angles = (0, 0) if rot is None else (rot.shape[1], rot.shape[0])
+    a = PagedAppendArgs(cache, qkv.data_ptr(), qkv.stride(0), _ptr(q_norm), _ptr(k_norm), _ptr(rot), 2 * half, angles, pairs, _ptr(positions), seqs.data_ptr(), slots.data_ptr(),
+                        _ptr(q), heads * cache.dim, qkv.shape[0], heads, eps, _ptr(status))
     _check(lib().glmb_paged_append(C.byref(a), _stream()), "paged_append")
 
 
-def tree_attention(q, k, v, table, starts, lengths, masks, scale, max_rows, sink, out, *, clear_rest=False, status=None):
+def tree_attention(q, cache: PagedArgs, starts, lengths, masks, scale, max_rows, sink, out, *, clear_rest=False, status=None):
     """Attention of drafted rows over a paged cache and their ancestors (``layers.attention.paged.tree_attention``)."""
     rows, H, _ = q.shape
-    a = TreeAttentionArgs(_paged(k, v, table), q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), starts.data_ptr(), lengths.data_ptr(),
-                          masks.data_ptr(), None if sink is None else sink.data_ptr(), None, None, 0, rows, H, max_rows, scale, int(clear_rest),
-                          None if status is None else status.data_ptr())
-    lib()
+    q_row, q_head, _ = q.stride()
+    out_row, out_head, _ = out.stride()
+    a = TreeAttentionArgs(cache, q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, starts.data_ptr(), lengths.data_ptr(), masks.data_ptr(), _ptr(sink), None, None, 0,
+                          rows, H, max_rows, scale, clear_rest, _ptr(status))
+    launch = lib().glmb_tree_attention
     parts = _lib.glmb_tree_attention_parts(C.byref(a))  # not a launch: past the wrapper that times launches
-    vdim = v.shape[3]
-    room = torch.empty(max(parts, 0) * (vdim + 2), dtype=torch.float32, device=q.device)  # sums of keys that several CTAs share
-    a.part_o, a.part_ml, a.parts = room.data_ptr(), room.data_ptr() + 4 * parts * vdim, parts
-    _check(lib().glmb_tree_attention(C.byref(a), _stream()), "tree_attention")
+    if parts < 0:
+        raise ValueError("tree_attention: sizes that the kernels do not take")
+    room = torch.empty(parts * (cache.vdim + 2), dtype=torch.float32, device=q.device)  # sums of keys that several CTAs share
+    a.part_o = room.data_ptr()
+    a.part_ml, a.parts = a.part_o + 4 * parts * cache.vdim, parts
+    _check(launch(C.byref(a), _stream()), "tree_attention")
 
 
 def fp8_to_bf16(bits, scale, out, block=(128, 128), status=None):

@@ -36,7 +36,7 @@ def test_rows_without_probabilities():
 def test_refusals():
     x, t = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
     for bad in (lambda: logprobs.token_logprobs(x.double(), t), lambda: logprobs.token_logprobs(x[0], t), lambda: logprobs.token_logprobs(x, t[:1]), lambda: logprobs.token_logprobs(x, t.float()),
-                lambda: logprobs.token_logprobs(x, t, top=6), lambda: logprobs.token_logprobs(x, t, top=-1), lambda: logprobs.token_logprobs(torch.zeros(2, 50), t, top=33),
+                lambda: logprobs.token_logprobs(x, t, top=6), lambda: logprobs.token_logprobs(x, t, status=torch.zeros(1)), lambda: logprobs.token_logprobs(x, t, status=torch.zeros(2, dtype=torch.int32)), lambda: logprobs.token_logprobs(x, t, top=-1), lambda: logprobs.token_logprobs(torch.zeros(2, 50), t, top=33),
                 lambda: logprobs.token_logprobs(torch.zeros(2, 0), t), lambda: logprobs.head_logprobs(x, torch.zeros(7, 4), t), lambda: logprobs.head_logprobs(x, torch.zeros(7, 5).bfloat16(), t),
                 lambda: logprobs.head_logprobs(x, torch.zeros(7, 5), t, vocab=8), lambda: logprobs.head_logprobs(x, torch.zeros(7, 5), t, vocab=0)):
         with pytest.raises(ValueError):

@@ -70,13 +70,13 @@ def test_refusals():
     c = case["cache"]
     cut = lambda **more: lambda: paged.tree_attention(**(case | more))  # noqa: E731
     bad = [cut(q=case["q"].float()), cut(q=case["q"][:, :3]), cut(q=case["q"][..., :8]), cut(starts=case["starts"].long()), cut(starts=case["starts"][:1]), cut(lengths=case["starts"]),
-           cut(masks=case["masks"].int()), cut(masks=case["masks"][:1]), cut(max_rows=0), cut(max_rows=65), cut(scale=0.0), cut(scale=-1.0), cut(scale=float("nan")), cut(cache=paged.PagedKV(c.k[:, :4], c.v[:, :4], c.table)), cut(cache=paged.PagedKV(c.k[:0], c.v[:0], c.table)), cut(sink=torch.zeros(3)), cut(sink=torch.zeros(4).double()),
+           cut(masks=case["masks"].int()), cut(masks=case["masks"][:1]), cut(max_rows=0), cut(max_rows=65), cut(scale=0.0), cut(scale=-1.0), cut(scale=float("nan")), cut(cache=paged.PagedKV(c.k[:, :4], c.v[:, :4], c.table)), cut(cache=paged.PagedKV(c.k[:0], c.v[:0], c.table)), cut(sink=torch.zeros(3)), cut(status=torch.zeros(2, dtype=torch.int32)), cut(status=torch.zeros(1)), cut(sink=torch.zeros(4).double()),
            cut(cache=paged.PagedKV(c.k.float(), c.v, c.table)), cut(cache=paged.PagedKV(c.k, c.v[:1], c.table)), cut(cache=paged.PagedKV(c.k, c.v, c.table.long())),
            cut(cache=paged.PagedKV(c.k[..., :8], c.v, c.table)), cut(cache=paged.PagedKV(c.k, c.v, c.table[0])), cut(out=torch.zeros(2, 4, 8).bfloat16())]
     qkv, one = torch.zeros(2, 4 * 16 + 4 * 16).bfloat16(), torch.zeros(2, dtype=torch.int32)
     rot = torch.zeros(9, 8, 2)
     app = lambda *a, **more: lambda: paged.append(*(a or (qkv, c, one, one, one)), **({"heads": 4} | more))  # noqa: E731
-    bad += [app(heads=3), app(heads=0), app(qkv.float(), c, one, one, one), app(qkv, c, one, one[:1], one), app(qkv, c, one, one, one.long()), app(qkv, c, None, one, one, rot=rot),
+    bad += [app(status=torch.zeros(1)), app(heads=3), app(heads=0), app(qkv.float(), c, one, one, one), app(qkv, c, one, one[:1], one), app(qkv, c, one, one, one.long()), app(qkv, c, None, one, one, rot=rot),
             app(rot=rot.double()), app(rot=torch.zeros(9, 9, 2)), app(rot=torch.zeros(9, 0, 2)), app(q_norm=torch.ones(16)), app(k_norm=torch.ones(8).bfloat16())]
     for call in bad:
         with pytest.raises(ValueError):
