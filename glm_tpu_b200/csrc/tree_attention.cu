@@ -16,6 +16,9 @@
 //   softmax         128 threads, one row each, running maximum and sum in fp32; weights back into TMEM where the scores were, in bf16
 //   O += P V        A = weights from TMEM, B = values as they lie in memory
 //
+// A tile of up to 64 or 32 pairs is there two or four times among the 128 rows: each copy weighs its own half or quarter of every block (its weights of the rest
+// are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs.
+//
 // The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
 // (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-9 beside that of the result.
 // A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; memory is its bound, so its weights
@@ -29,7 +32,7 @@
 // (out of the tensor map's range) or cleared in shared memory before the product; drafted values that are not finite are cleared too, and the rows
 // that do see them add their product afterwards, one by one.
 //
-// Runs that share a unit leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.
+// Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.
 // Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -38,6 +41,7 @@
 #define TA_LOG2E 1.4426950408889634f
 #define TA_MAX_DRAFTS 64  // bits of a mask
 #define TA_THREADS 320
+#define TM_WARPS 8
 #define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
 #define TA_NOTES 8        // blocks whose pages are remembered: the producer is at most five ahead of the softmax
 
@@ -62,22 +66,12 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttentionArgs& a, int b, b
 
 // How units are made: `heads` of a tile (of `head_blocks` of a key head), `tile_rows` drafted rows of a tile, tiles of a unit.
 struct TreeShape {
-    int per, heads, head_blocks, tile_rows, in_unit, keys, ctas, units_max;  // units_max: of a key head of the largest sequence
+    int per, heads, head_blocks, tile_rows, in_unit, copies, keys, ctas, units_max;  // units_max: of a key head of the largest sequence
+    // The place of a tile's sums of a segment; a row's lie behind it.
+    __device__ __forceinline__ int64_t part(int64_t segment, int tile_of_unit, int copy) const { return ((segment * in_unit + tile_of_unit) * copies + copy) * (heads * tile_rows); }
     __device__ __forceinline__ int tiles(int rows) const { return (rows + tile_rows - 1) / tile_rows * head_blocks; }
     __device__ __forceinline__ int units(int rows) const { return (tiles(rows) + in_unit - 1) / in_unit; }
 };
-
-// Blocks of all sequences before sequence b (`upto` = seqs: all); the whole warp.
-__device__ __forceinline__ int64_t tree_blocks(const TreeAttentionArgs& a, const TreeShape& sh, int upto, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < upto; b += 32) {
-        const TreeSeq s = tree_seq(a, b, false);
-        sum += (int64_t)s.blocks(sh.keys) * sh.units(s.rows) * a.cache.G;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
-}
 
 // The part of a CTA's run that lies in one unit.
 struct TreeSegment {
@@ -152,18 +146,19 @@ __device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
     return (uint32_t)(mask << -ahead) | ((1u << -ahead) - 1u);
 }
 
-template <int MODE> struct TreeMode {
+template <int MODE, int COPIES> struct TreeMode {
+    static constexpr int ROWS = 128 / COPIES, COLS = (MODE == TA_WIDE ? 64 : 128) / COPIES;  // rows of the tile, keys of a block that a thread weighs
     static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2;
     static constexpr int STAGES = MODE == TA_SINGLE ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
     static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
     static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + 1024;
 };
 
-template <int MODE>
+template <int MODE, int COPIES>
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh, int slots_first_k, int slots_first_v, int chunk) {
-    typedef TreeMode<MODE> T;
+    typedef TreeMode<MODE, COPIES> T;
     constexpr int KEYS = T::KEYS, STAGES = T::STAGES, WORDS = KEYS / 32;
     GLMB_PDL_PROLOGUE();  // before the TMEM allocation: a kernel still running may need the columns to finish
     extern __shared__ unsigned char smem_raw[];
@@ -195,16 +190,20 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (warp == 9) {  // this CTA's run: equal numbers of blocks, in the order of the sequences
-        const int64_t total = tree_blocks(a, sh, c.seqs, lane), share = (total + sh.ctas - 1) / sh.ctas;
-        const int64_t first = min(total, share * (int)blockIdx.x), count = min(share, total - first);
+        auto blocks_of = [&](int b) {
+            if (b >= c.seqs) return (int64_t)0;
+            const TreeSeq s = tree_seq(a, b, blockIdx.x == 0);
+            return (int64_t)s.blocks(KEYS) * sh.units(s.rows) * c.G;
+        };
+        int64_t mine = blocks_of(lane), total = mine;
+        for (int b = lane + 32; b < c.seqs; b += 32) total += blocks_of(b);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const int64_t share = (total + sh.ctas - 1) / sh.ctas, first = min(total, share * (int)blockIdx.x), count = min(share, total - first);
         int64_t before = 0;
-        int seq = 0, found = -1;
-        for (; seq < c.seqs && found < 0; seq += 32) {
-            int64_t mine = 0;
-            if (seq + lane < c.seqs) {
-                const TreeSeq s = tree_seq(a, seq + lane, blockIdx.x == 0);
-                mine = (int64_t)s.blocks(KEYS) * sh.units(s.rows) * c.G;
-            }
+        int found = -1;
+        for (int seq = 0; seq < c.seqs && found < 0; seq += 32) {
+            if (seq > 0) mine = blocks_of(seq + lane);
             int64_t upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -219,8 +218,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (blockIdx.x == 0)
-            for (int b = seq + lane; b < c.seqs; b += 32) tree_seq(a, b, true);  // the report on those not looked at
         if (lane == 0) run_s[0] = found < 0 ? 0 : count;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -253,11 +250,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (lane == 0) broken[segment & 3] = 0;
             __syncwarp();
             if (elect_one()) {
-                mbar_expect_tx(&q_full, tiles * kboxes * sh.heads * sh.tile_rows * 128);
+                mbar_expect_tx(&q_full, tiles * kboxes * COPIES * sh.heads * sh.tile_rows * 128);
                 for (int t = 0; t < tiles; ++t) {
                     const int tile = s.unit * sh.in_unit + t;
-                    for (int x = 0; x < kboxes; ++x)
-                        ta_tma_3d(q_s + (t * kboxes + x) * T::Q_BOX, &map_q, &q_full, x * 64, s.g * sh.per + tile % sh.head_blocks * sh.heads,
+                    for (int x = 0; x < kboxes * COPIES; ++x)
+                        ta_tma_3d(q_s + (t * kboxes + x / COPIES) * T::Q_BOX + x % COPIES * T::ROWS * 128, &map_q, &q_full, x / COPIES * 64, s.g * sh.per + tile % sh.head_blocks * sh.heads,
                                   s.seq.row0 + tile / sh.head_blocks * sh.tile_rows);
                 }
             }
@@ -350,7 +347,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
         }
     } else {
-        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, copy = row / T::ROWS, in = row % T::ROWS, col0 = copy * T::COLS;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_addr = tmem + t * 128 + lanes;
         const float scale2 = a.scale * TA_LOG2E;
         const bool fixes = MODE != TA_PAIR || t == 0;  // of two tiles the first one's products come first
@@ -363,8 +360,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 continue;
             }
             const int tile = s.unit * sh.in_unit + (MODE == TA_PAIR ? t : 0), j0 = tile / sh.head_blocks * sh.tile_rows, h0 = tile % sh.head_blocks * sh.heads;
-            const int j = j0 + row / sh.heads, hh = h0 + row % sh.heads;
-            const bool live = row < sh.heads * sh.tile_rows && j < s.seq.rows && hh < sh.per, warp_live = __any_sync(0xffffffffu, live);
+            const int j = j0 + in / sh.heads, hh = h0 + in % sh.heads;
+            const bool live = in < sh.heads * sh.tile_rows && j < s.seq.rows && hh < sh.per, warp_live = __any_sync(0xffffffffu, live);
             const uint64_t drafts = s.seq.drafts >= 64 ? ~0ull : (1ull << s.seq.drafts) - 1ull;
             const uint64_t mask = live ? (uint64_t)a.masks[s.seq.row0 + j] & drafts : 0;
             float m = -INFINITY, l = 0.f;
@@ -379,23 +376,30 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 for (int w = 0; w < WORDS; ++w) there &= page_bits[number % TA_NOTES][w];
                 const bool drafted = base + KEYS > s.seq.length;
                 if (warp_live) {
-                    uint32_t x[KEYS];
+                    float x[T::COLS];
+                    constexpr int PARTS = (T::COLS + 31) / 32;  // loads of 32 columns
 #pragma unroll
-                    for (int i = 0; i < WORDS; ++i) ta_tmem_ld32_nowait(s_addr + i * 32, x + i * 32);
+                    for (int i = 0; i < PARTS; ++i) ta_tmem_ld32_nowait(s_addr + col0 + i * 32, reinterpret_cast<uint32_t*>(x) + i * 32);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (drafted || there != ~0u) {
 #pragma unroll
-                        for (int w = 0; w < WORDS; ++w) {
-                            const uint32_t sees = ta_visible(base + w * 32 - s.seq.length, mask) & page_bits[number % TA_NOTES][w];
+                        for (int w = 0; w < PARTS; ++w) {
+                            const uint32_t sees = ta_visible(base + col0 + w * 32 - s.seq.length, mask) & page_bits[number % TA_NOTES][col0 / 32 + w];
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (!(sees >> i & 1)) x[w * 32 + i] = 0xff800000u;  // -infinity
+                                if (!(sees >> i & 1)) x[w * 32 + i] = -INFINITY;
                         }
                     }
-                    float top[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+                    float top[8];
 #pragma unroll
-                    for (int i = 4; i < KEYS; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    for (int i = 0; i < 8; ++i) top[i] = x[i];
+#pragma unroll
+                    for (int i = 8; i < T::COLS; ++i) top[i & 7] = fmaxf(top[i & 7], x[i]);
+#pragma unroll
+                    for (int i = 4; i > 0; i >>= 1)
+#pragma unroll
+                        for (int e = 0; e < i; ++e) top[e] = fmaxf(top[e], top[e + i]);
+                    const float most = top[0] * scale2;
                     if (n == 0) {
                         m = most;
                     } else if (__any_sync(0xffffffffu, most > m + TA_SLACK)) {
@@ -411,22 +415,33 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         }
                     }
                     const float from = m == -INFINITY ? 0.f : m;
-                    float sum0 = 0.f, sum1 = 0.f;
+                    const float2 scale_2 = make_float2(scale2, scale2), from_2 = make_float2(-from, -from);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int w = 0; w < WORDS; ++w) {
+                    for (int w = 0; w < PARTS; ++w) {
                         uint32_t hi[16], lo[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float p = ta_exp2(fmaf(__uint_as_float(x[w * 32 + 2 * i]), scale2, -from)), r = ta_exp2(fmaf(__uint_as_float(x[w * 32 + 2 * i + 1]), scale2, -from));
-                            sum0 += p;
-                            sum1 += r;
-                            hi[i] = pack_bf16(p, r);
-                            if (T::PIECES == 2) lo[i] = pack_bf16(p - bf16_lo(hi[i]), r - bf16_hi(hi[i]));
+                            const float2 z = __ffma2_rn(make_float2(x[w * 32 + 2 * i], x[w * 32 + 2 * i + 1]), scale_2, from_2), p = make_float2(ta_exp2(z.x), ta_exp2(z.y));
+                            sum[i & 1] = __fadd2_rn(sum[i & 1], p);
+                            hi[i] = pack_bf16(p.x, p.y);
+                            if (T::PIECES == 2) {
+                                const float2 rest = __fadd2_rn(p, make_float2(-bf16_lo(hi[i]), -bf16_hi(hi[i])));
+                                lo[i] = pack_bf16(rest.x, rest.y);
+                            }
                         }
-                        ta_tmem_st16(s_addr + w * 16, hi);
-                        if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + w * 16, lo);
+                        ta_tmem_st16(s_addr + col0 / 2 + w * 16, hi);
+                        if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + col0 / 2 + w * 16, lo);
                     }
-                    l += sum0 + sum1;
+                    if constexpr (COPIES > 1) {  // the other copies' keys are not this row's
+                        const uint32_t none[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                        for (int at = 0; at < KEYS / 2; at += 16)
+                            if (at < col0 / 2 || at >= col0 / 2 + T::COLS / 2) {
+                                ta_tmem_st16(s_addr + at, none);
+                                if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + at, none);
+                            }
+                    }
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 if (drafted && fixes) {  // values that nobody, or not everybody, may multiply
@@ -471,7 +486,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t lost = broken[segment & 3] & mask;
-            const bool whole = s.blocks == s.of;  // no other CTA has keys of this unit
+            const bool whole = COPIES == 1 && s.blocks == s.of;  // nobody else has keys of this row
             if (warp_live) {
                 float f0 = 1.f, f1 = 0.f;
                 if (both) {
@@ -493,7 +508,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 bf16* dst = a.out + (int64_t)out_row * a.out_row + (int64_t)head * a.out_head;
                 const int64_t slot = ((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x;
-                const int64_t part = (slot * sh.in_unit + (MODE == TA_PAIR ? t : 0)) * (sh.heads * sh.tile_rows) + row;
+                const int64_t part = sh.part(slot, MODE == TA_PAIR ? t : 0, copy) + in;
                 for (int x0 = 0; x0 < c.vdim; x0 += 16) {
                     uint32_t o[16];
                     tmem_ld16(tmem + 256 + t * 128 + lanes + x0, o);
@@ -508,6 +523,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (!live) continue;
                     for (uint64_t left = lost; left; left &= left - 1) {  // drafted values that were left out of the product
                         const int drafted_slot = s.seq.length + __ffsll(left) - 1, page = paged_page(c, s.b, drafted_slot);
+                        if (drafted_slot % KEYS / T::COLS != copy) continue;
                         const bf16* k = c.k + page * c.k_page + (drafted_slot % c.page) * c.k_slot + s.g * c.k_head;
                         const bf16* v = c.v + page * c.v_page + (drafted_slot % c.page) * c.v_slot + s.g * c.v_head + x0;
                         const bf16* q = a.q + (int64_t)out_row * a.q_row + (int64_t)head * a.q_head;
@@ -550,60 +566,93 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
 }
 
-// One CTA a row: joins the sums that several runs left of its heads, or clears the row where it belongs to no sequence.
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh) {
+// A warp a row and head: joins the sums that several runs or copies left, or clears the row where it belongs to no sequence.  grid (rows, blocks of heads).
+__global__ void __launch_bounds__(TM_WARPS * 32) tree_merge_kernel(const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh) {
     GLMB_PDL_PROLOGUE();
-    __shared__ int64_t before_s[2];
     const PagedArgs& c = a.cache;
-    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int low = 0, high = c.seqs;  // the last sequence that begins at or before the row
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (a.starts[mid] <= row) low = mid;
-        else high = mid;
+    const int row = blockIdx.x, h = blockIdx.y * TM_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (h >= a.H) return;
+    // the row's sequence is the last that begins at or before it; blocks of all sequences, and of those that begin no later
+    int64_t total = 0, upto = 0;
+    int b = -1;
+    for (int b0 = 0; b0 < c.seqs; b0 += 32) {
+        bool begun = false;
+        if (b0 + lane < c.seqs) {
+            const TreeSeq s = tree_seq(a, b0 + lane, false);
+            const int64_t mine = (int64_t)s.blocks(sh.keys) * sh.units(s.rows) * c.G;
+            begun = a.starts[b0 + lane] <= row;
+            total += mine;
+            upto += begun ? mine : 0;
+        }
+        b += __popc(__ballot_sync(0xffffffffu, begun));
     }
-    const int b = low;
-    const TreeSeq seq = tree_seq(a, b, false);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        upto += __shfl_xor_sync(0xffffffffu, upto, o);
+    }
+    bf16* dst = a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head;
+    TreeSeq seq{0, 0, 0, 0};
+    if (b >= 0) seq = tree_seq(a, b, false);
     const int j = row - seq.row0;
-    if (j < 0 || j >= seq.rows) {
+    if (b < 0 || j < 0 || j >= seq.rows) {
         if (a.clear_rest)
-            for (int i = threadIdx.x; i < a.H * (c.vdim >> 3); i += 256) {
-                const int h = i / (c.vdim >> 3), d = i % (c.vdim >> 3) * 8;
-                *reinterpret_cast<uint4*>(a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head + d) = make_uint4(0, 0, 0, 0);
-            }
+            for (int d = lane * 8; d < c.vdim; d += 256) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
         return;
     }
-    if (warp < 2) {
-        const int64_t sum = tree_blocks(a, sh, warp == 0 ? c.seqs : b, lane);
-        if (lane == 0) before_s[warp] = sum;
-    }
-    __syncthreads();
-    const int64_t share = (before_s[0] + sh.ctas - 1) / sh.ctas;
-    const int blocks = seq.blocks(sh.keys), units = sh.units(seq.rows);
-    const int pieces = c.vdim >> 2;  // of four columns
-    for (int i = threadIdx.x; i < a.H * pieces; i += 256) {
-        const int h = i / pieces, d = i % pieces * 4, g = h / sh.per, hh = h % sh.per;
-        const int tile = j / sh.tile_rows * sh.head_blocks + hh / sh.heads, unit = tile / sh.in_unit;
-        const int64_t from = before_s[1] + ((int64_t)g * units + unit) * blocks;
-        const int first = (int)(from / share), last = (int)((from + blocks - 1) / share);  // CTAs with keys of the unit
-        if (first == last) continue;  // written already
-        const int64_t slot = ((int64_t)b * c.G + g) * sh.units_max + unit, in = j % sh.tile_rows * sh.heads + hh % sh.heads;
-        auto part = [&](int cta) { return ((slot + cta) * sh.in_unit + tile % sh.in_unit) * (sh.heads * sh.tile_rows) + in; };
-        float m = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int cta = first; cta <= last; ++cta) {
-            const int64_t p = part(cta);
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
-            const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * c.vdim + d);
-            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing there
-            const float next = fmaxf(m, ml.x), f0 = m == next ? 1.f : ta_exp2(m - next), f1 = ml.x == next ? 1.f : ta_exp2(ml.x - next);
-            m = next;
-            l = l * f0 + ml.y * f1;
-            o[0] = o[0] * f0 + v.x * f1, o[1] = o[1] * f0 + v.y * f1, o[2] = o[2] * f0 + v.z * f1, o[3] = o[3] * f0 + v.w * f1;
+    const int64_t share = (total + sh.ctas - 1) / sh.ctas;
+    const int blocks = seq.blocks(sh.keys), units = sh.units(seq.rows), g = h / sh.per, hh = h % sh.per;
+    const int tile = j / sh.tile_rows * sh.head_blocks + hh / sh.heads, unit = tile / sh.in_unit;
+    const int64_t from = upto - (int64_t)blocks * units * c.G + ((int64_t)g * units + unit) * blocks;
+    const int first = (int)(from / share), last = (int)((from + blocks - 1) / share), parts = (last - first + 1) * sh.copies;  // CTAs with keys of the unit
+    if (parts == 1) return;  // written already
+    const int64_t slot = ((int64_t)b * c.G + g) * sh.units_max + unit + first;
+    const int in = j % sh.tile_rows * sh.heads + hh % sh.heads;
+    auto place = [&](int k) { return sh.part(slot + k / sh.copies, tile % sh.in_unit, k % sh.copies) + in; };
+    float m = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;  // the same in every lane
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // columns 4 lane .. and 128 + 4 lane ..
+    const int d0 = lane * 4, d1 = 128 + lane * 4;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (k0 + lane < parts) ml = *reinterpret_cast<const float2*>(a.part_ml + place(k0 + lane) * 2);
+        const bool empty = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing there
+        const float next = fmaxf(m, warp_max(ml.x)), fix = m == next ? 1.f : ta_exp2(m - next);
+        const float w = empty ? 0.f : ml.x == next ? 1.f : ta_exp2(ml.x - next);
+        m = next;
+        l = l * fix + warp_sum(empty ? 0.f : ml.y * w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] *= fix;
+        const int here = min(32, parts - k0);
+        const int64_t at = k0 + lane < parts ? place(k0 + lane) * c.vdim : 0;
+        for (int k = 0; k < here; k += 8) {  // eight on their way; an empty sum is zeros
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int64_t from_k = __shfl_sync(0xffffffffu, at, k + u);
+                v[u] = k + u < here && d0 < c.vdim ? *reinterpret_cast<const float4*>(a.part_o + from_k + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float wk = __shfl_sync(0xffffffffu, w, k + u);
+                o[0] = fmaf(wk, v[u].x, o[0]), o[1] = fmaf(wk, v[u].y, o[1]), o[2] = fmaf(wk, v[u].z, o[2]), o[3] = fmaf(wk, v[u].w, o[3]);
+            }
+            if (c.vdim > 128) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int64_t from_k = __shfl_sync(0xffffffffu, at, k + u);
+                    v[u] = k + u < here && d1 < c.vdim ? *reinterpret_cast<const float4*>(a.part_o + from_k + d1) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float wk = __shfl_sync(0xffffffffu, w, k + u);
+                    o[4] = fmaf(wk, v[u].x, o[4]), o[5] = fmaf(wk, v[u].y, o[5]), o[6] = fmaf(wk, v[u].z, o[6]), o[7] = fmaf(wk, v[u].w, o[7]);
+                }
+            }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>(a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d0 < c.vdim) *reinterpret_cast<uint2*>(dst + d0) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+    if (d1 < c.vdim) *reinterpret_cast<uint2*>(dst + d1) = make_uint2(pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
@@ -616,6 +665,8 @@ static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
     const int tiles = ceil_div(a.max_rows, sh.tile_rows) * sh.head_blocks;
     mode = a.cache.dim > 128 || a.cache.vdim > 128 ? TA_WIDE : tiles > 1 ? TA_PAIR : TA_SINGLE;
     sh.in_unit = mode == TA_PAIR ? 2 : 1;
+    const int tile = sh.heads * sh.tile_rows;
+    sh.copies = mode == TA_PAIR || tile > 64 ? 1 : tile > 32 || mode == TA_WIDE ? 2 : 4;
     sh.keys = mode == TA_WIDE ? 64 : 128;
     sh.ctas = 148;
     sh.units_max = ceil_div(tiles, sh.in_unit);
@@ -623,7 +674,7 @@ static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
 }
 // Sums that all segments may leave: one for each unit and one more for each CTA.
 static int64_t tree_parts(const TreeAttentionArgs& a, const TreeShape& sh) {
-    return ((int64_t)a.cache.seqs * a.cache.G * sh.units_max + sh.ctas) * sh.in_unit * sh.heads * sh.tile_rows;
+    return ((int64_t)a.cache.seqs * a.cache.G * sh.units_max + sh.ctas) * sh.in_unit * sh.copies * sh.heads * sh.tile_rows;
 }
 static int tree_refuses(const TreeAttentionArgs& a) {
     const PagedArgs& c = a.cache;
@@ -650,9 +701,9 @@ static int tree_query_map(CUtensorMap* map, const TreeAttentionArgs& a, const Tr
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
 }
 
-template <int MODE>
+template <int MODE, int COPIES>
 static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStream_t stream) {
-    typedef TreeMode<MODE> T;
+    typedef TreeMode<MODE, COPIES> T;
     int chunk = 8;  // slots that lie in one page wherever a block begins
     while (chunk < T::KEYS && a.cache.page % (2 * chunk) == 0) chunk *= 2;
     const PagedArgs& c = a.cache;
@@ -664,14 +715,14 @@ static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStre
     static DeviceOnce once;
     const int dev = once.pending();
     if (dev != DeviceOnce::SET) {
-        const cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute((const void*)tree_attention_kernel<MODE, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
         if (e != cudaSuccess) return (int)e;
         once.mark(dev);
     }
-    GLMB_LAUNCH(tree_attention_kernel<MODE>, sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
+    GLMB_LAUNCH((tree_attention_kernel<MODE, COPIES>), sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
-    GLMB_LAUNCH(tree_merge_kernel, a.rows, 256, 0, stream, a, sh);
+    GLMB_LAUNCH(tree_merge_kernel, dim3(a.rows, ceil_div(a.H, TM_WARPS)), TM_WARPS * 32, 0, stream, a, sh);
     return (int)cudaGetLastError();
 }
 
@@ -692,5 +743,7 @@ GLMB_API int glmb_tree_attention(const TreeAttentionArgs* args, cudaStream_t str
     int mode;
     const TreeShape sh = tree_shape(a, mode);
     if (a.parts < tree_parts(a, sh) || !a.part_o || !a.part_ml) return 1;
-    return mode == TA_PAIR ? tree_launch<TA_PAIR>(a, sh, stream) : mode == TA_SINGLE ? tree_launch<TA_SINGLE>(a, sh, stream) : tree_launch<TA_WIDE>(a, sh, stream);
+    if (mode == TA_PAIR) return tree_launch<TA_PAIR, 1>(a, sh, stream);
+    if (mode == TA_WIDE) return sh.copies == 1 ? tree_launch<TA_WIDE, 1>(a, sh, stream) : tree_launch<TA_WIDE, 2>(a, sh, stream);
+    return sh.copies == 1 ? tree_launch<TA_SINGLE, 1>(a, sh, stream) : sh.copies == 2 ? tree_launch<TA_SINGLE, 2>(a, sh, stream) : tree_launch<TA_SINGLE, 4>(a, sh, stream);
 }
