@@ -26,7 +26,7 @@
 //
 //   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
 //   warp 8           issues every tcgen05.mma, owns the TMEM allocation
-//   warp 9           looks pages up, brings queries, keys and values in by TMA
+//   warps 9, 10      look pages up, bring queries and keys, and values, in by TMA
 //
 // What a row does not see must not reach it, and a weight of zero times NaN is NaN.  Slots behind the last one, and pages that do not exist, are read as zeros
 // (out of the tensor map's range) or cleared in shared memory before the product; drafted values that are not finite are cleared too, and the rows
@@ -40,7 +40,7 @@
 
 #define TA_LOG2E 1.4426950408889634f
 #define TA_MAX_DRAFTS 64  // bits of a mask
-#define TA_THREADS 320
+#define TA_THREADS 352
 #define TM_WARPS 8
 #define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
 #define TA_NOTES 8        // blocks whose pages are remembered: the producer is at most five ahead of the softmax
@@ -242,55 +242,58 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     TreeSegment s;
     uint32_t gone = 0;  // blocks of the segments before this one
     int segment = 0;
-    if (warp == 9) {
+    if (warp >= 9) {  // keys (and queries), values
+        const bool keys = warp == 9;
+        const int boxes = keys ? kboxes : vboxes, chunks = KEYS / chunk;
+        const CUtensorMap* map = keys ? &map_k : &map_v;
+        const bool slots_first = keys ? slots_first_k : slots_first_v;
+        unsigned char* ring = keys ? k_s : v_s;
+        uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
         bool ok = true;
         for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
-            if (segment > 0 && !mbar_wait_warp(&q_empty, (segment - 1) & 1)) { fail = 1; break; }
-            const int tiles = MODE == TA_PAIR ? min(2, sh.tiles(s.seq.rows) - s.unit * 2) : 1;
-            if (lane == 0) broken[segment & 3] = 0;
-            __syncwarp();
-            if (elect_one()) {
-                mbar_expect_tx(&q_full, tiles * kboxes * COPIES * sh.heads * sh.tile_rows * 128);
-                for (int t = 0; t < tiles; ++t) {
-                    const int tile = s.unit * sh.in_unit + t;
-                    for (int x = 0; x < kboxes * COPIES; ++x)
-                        ta_tma_3d(q_s + (t * kboxes + x / COPIES) * T::Q_BOX + x % COPIES * T::ROWS * 128, &map_q, &q_full, x / COPIES * 64, s.g * sh.per + tile % sh.head_blocks * sh.heads,
-                                  s.seq.row0 + tile / sh.head_blocks * sh.tile_rows);
+            if (keys) {
+                if (segment > 0 && !mbar_wait_warp(&q_empty, (segment - 1) & 1)) { fail = 1; break; }
+                const int tiles = MODE == TA_PAIR ? min(2, sh.tiles(s.seq.rows) - s.unit * 2) : 1;
+                if (lane == 0) broken[segment & 3] = 0;
+                __syncwarp();
+                if (elect_one()) {
+                    mbar_expect_tx(&q_full, tiles * kboxes * COPIES * sh.heads * sh.tile_rows * 128);
+                    for (int t = 0; t < tiles; ++t) {
+                        const int tile = s.unit * sh.in_unit + t;
+                        for (int x = 0; x < kboxes * COPIES; ++x)
+                            ta_tma_3d(q_s + (t * kboxes + x / COPIES) * T::Q_BOX + x % COPIES * T::ROWS * 128, &map_q, &q_full, x / COPIES * 64,
+                                      s.g * sh.per + tile % sh.head_blocks * sh.heads, s.seq.row0 + tile / sh.head_blocks * sh.tile_rows);
+                    }
                 }
+                __syncwarp();
             }
-            __syncwarp();
-            const int chunks = KEYS / chunk, last = s.seq.length + s.seq.drafts;  // slots from `last` on hold nothing
+            const int last = s.seq.length + s.seq.drafts;  // slots from `last` on hold nothing
             auto page_of = [&](int block) {  // lane i: the page of the i-th chunk, or one behind the last (read as zeros)
                 const int slot = (s.block0 + block) * KEYS + lane * chunk;
                 if (block >= s.blocks || lane >= chunks || slot >= last) return c.pages;
                 const int page = paged_page(c, s.b, slot);
-                if (page < 0) raise_status(a.status, GLMB_STATUS_BAD_INDEX);
+                if (page < 0 && keys) raise_status(a.status, GLMB_STATUS_BAD_INDEX);
                 return page < 0 ? c.pages : page;
             };
             int page = page_of(0);
             for (int j = 0; j < s.blocks; ++j) {
                 const uint32_t n = gone + j, st = n % STAGES, lap = n / STAGES;
-                const int next_page = page_of(j + 1), slot = (s.block0 + j) * KEYS + lane * chunk, in_page = slot % c.page;
-                if (lap > 0 && !mbar_wait_warp(k_empty + st, (lap - 1) & 1)) { fail = 1; ok = false; break; }
-                const uint32_t there = __ballot_sync(0xffffffffu, page < c.pages);
-                if (lane < WORDS) {
-                    uint32_t bits = 0;
-                    for (int i = 0; i < 32; i += 8) bits |= there >> ((lane * 32 + i) / chunk) & 1u ? 0xffu << i : 0u;
-                    page_bits[n % TA_NOTES][lane] = bits;
+                const int next_page = page_of(j + 1), in_page = ((s.block0 + j) * KEYS + lane * chunk) % c.page;
+                if (lap > 0 && !mbar_wait_warp(empty + st, (lap - 1) & 1)) { fail = 1; ok = false; break; }
+                if (keys) {
+                    const uint32_t there = __ballot_sync(0xffffffffu, page < c.pages);
+                    if (lane < WORDS) {
+                        uint32_t bits = 0;
+                        for (int i = 0; i < 32; i += 8) bits |= there >> ((lane * 32 + i) / chunk) & 1u ? 0xffu << i : 0u;
+                        page_bits[n % TA_NOTES][lane] = bits;
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (lane == 0) mbar_expect_tx(k_full + st, kboxes * T::KV_BOX);  // releases the notes too
-                __syncwarp();
-                if (lane < chunks)
-                    for (int x = 0; x < kboxes; ++x)
-                        ta_tma_4d(k_s + (st * kboxes + x) * T::KV_BOX + lane * chunk * 128, &map_k, k_full + st, x * 64, slots_first_k ? in_page : s.g, slots_first_k ? s.g : in_page, page);
-                __syncwarp();
-                if (lap > 0 && !mbar_wait_warp(v_empty + st, (lap - 1) & 1)) { fail = 1; ok = false; break; }
-                if (lane == 0) mbar_expect_tx(v_full + st, vboxes * T::KV_BOX);
+                if (lane == 0) mbar_expect_tx(full + st, boxes * T::KV_BOX);  // releases the notes too
                 __syncwarp();
                 if (lane < chunks)
-                    for (int x = 0; x < vboxes; ++x)
-                        ta_tma_4d(v_s + (st * vboxes + x) * T::KV_BOX + lane * chunk * 128, &map_v, v_full + st, x * 64, slots_first_v ? in_page : s.g, slots_first_v ? s.g : in_page, page);
+                    for (int x = 0; x < boxes; ++x)
+                        ta_tma_4d(ring + (st * boxes + x) * T::KV_BOX + lane * chunk * 128, map, full + st, x * 64, slots_first ? in_page : s.g, slots_first ? s.g : in_page, page);
                 __syncwarp();
                 page = next_page;
             }
