@@ -17,7 +17,7 @@
 //   O += P V        A = weights from TMEM, B = values as they lie in memory
 //
 // A tile of up to 64 or 32 pairs is there two or four times among the 128 rows: each copy weighs its own half or quarter of every block (its weights of the rest
-// are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs.
+// are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs, or in shared memory.
 //
 // The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
 // (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-9 beside that of the result.
@@ -32,7 +32,9 @@
 // (out of the tensor map's range) or cleared in shared memory before the product; drafted values that are not finite are cleared too, and the rows
 // that do see them add their product afterwards, one by one.
 //
-// Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.
+// Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.  A cache of
+// at most four blocks a sequence is dealt in whole units and needs none (JOINS: the copies meet in shared memory, which costs a stage of the ring: 64 pairs
+// at 30,000 slots 109 us so, 103 otherwise): 36 requests of three tokens 22 -> 14.5 us, one token over 12 slots 14 -> 9.8.
 // Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -41,8 +43,9 @@
 #define TA_LOG2E 1.4426950408889634f
 #define TA_MAX_DRAFTS 64  // bits of a mask
 #define TA_THREADS 352
-#define TM_WARPS 8
 #define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
+#define TA_JOIN 68        // floats of a row of joined sums: 64 columns, padded
+#define TA_WHOLE_BLOCKS 4 // caches of so few blocks a sequence: units are not split
 #define TA_NOTES 8        // blocks whose pages are remembered: the producer is at most five ahead of the softmax
 
 enum { TA_PAIR = 0, TA_SINGLE = 1, TA_WIDE = 2 };
@@ -67,11 +70,40 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttentionArgs& a, int b, b
 // How units are made: `heads` of a tile (of `head_blocks` of a key head), `tile_rows` drafted rows of a tile, tiles of a unit.
 struct TreeShape {
     int per, heads, head_blocks, tile_rows, in_unit, copies, keys, ctas, units_max;  // units_max: of a key head of the largest sequence
+    int whole;  // runs are whole units, as many for every CTA: nothing is left to join
     // The place of a tile's sums of a segment; a row's lie behind it.
     __device__ __forceinline__ int64_t part(int64_t segment, int tile_of_unit, int copy) const { return ((segment * in_unit + tile_of_unit) * copies + copy) * (heads * tile_rows); }
+    // What a sequence's units count for in the runs.
+    __device__ __forceinline__ int64_t share_of(const TreeSeq& s, int G) const { return s.rows ? (int64_t)(whole ? 1 : s.blocks(keys)) * units(s.rows) * G : 0; }
     __device__ __forceinline__ int tiles(int rows) const { return (rows + tile_rows - 1) / tile_rows * head_blocks; }
     __device__ __forceinline__ int units(int rows) const { return (tiles(rows) + in_unit - 1) / in_unit; }
 };
+
+// Whose a row is: the last sequence that begins at or before it has it among its rows.  Also what the units of all sequences count for, and those of
+// the sequences that begin no later; the whole warp.
+struct TreeRow { TreeSeq seq; int b, j; bool mine; int64_t total, upto; };
+__device__ __forceinline__ TreeRow tree_row(const TreeAttentionArgs& a, const TreeShape& sh, int row, int lane) {
+    TreeRow r{{0, 0, 0, 0}, -1, 0, false, 0, 0};
+    for (int b0 = 0; b0 < a.cache.seqs; b0 += 32) {
+        bool begun = false;
+        if (b0 + lane < a.cache.seqs) {
+            const int64_t mine = sh.share_of(tree_seq(a, b0 + lane, false), a.cache.G);
+            begun = a.starts[b0 + lane] <= row;
+            r.total += mine;
+            r.upto += begun ? mine : 0;
+        }
+        r.b += __popc(__ballot_sync(0xffffffffu, begun));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        r.total += __shfl_xor_sync(0xffffffffu, r.total, o);
+        r.upto += __shfl_xor_sync(0xffffffffu, r.upto, o);
+    }
+    if (r.b >= 0) r.seq = tree_seq(a, r.b, false);
+    r.j = row - r.seq.row0;
+    r.mine = r.b >= 0 && r.j >= 0 && r.j < r.seq.rows;
+    return r;
+}
 
 // The part of a CTA's run that lies in one unit.
 struct TreeSegment {
@@ -95,8 +127,8 @@ struct TreeWalk {
                 continue;
             }
             s.b = b, s.g = at / units, s.unit = at % units, s.block0 = block0;
-            s.blocks = (int)min((int64_t)(s.of - block0), left);
-            left -= s.blocks;
+            s.blocks = sh.whole ? s.of : (int)min((int64_t)(s.of - block0), left);
+            left -= sh.whole ? 1 : s.blocks;
             ++at, block0 = 0;
             return true;
         }
@@ -146,21 +178,21 @@ __device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
     return (uint32_t)(mask << -ahead) | ((1u << -ahead) - 1u);
 }
 
-template <int MODE, int COPIES> struct TreeMode {
+template <int MODE, int COPIES, bool JOINS> struct TreeMode {
     static constexpr int ROWS = 128 / COPIES, COLS = (MODE == TA_WIDE ? 64 : 128) / COPIES;  // rows of the tile, keys of a block that a thread weighs
     static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2;
-    static constexpr int STAGES = MODE == TA_SINGLE ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
+    static constexpr int STAGES = MODE == TA_SINGLE && !JOINS ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
     static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
-    static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + 1024;
+    static constexpr int JOIN = JOINS ? 128 * TA_JOIN * 4 : 0;  // 64 columns of the copies' sums
+    static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + JOIN + 1024;
 };
 
-template <int MODE, int COPIES>
+template <int MODE, int COPIES, bool JOINS>
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh, int slots_first_k, int slots_first_v, int chunk) {
-    typedef TreeMode<MODE, COPIES> T;
+    typedef TreeMode<MODE, COPIES, JOINS> T;
     constexpr int KEYS = T::KEYS, STAGES = T::STAGES, WORDS = KEYS / 32;
-    GLMB_PDL_PROLOGUE();  // before the TMEM allocation: a kernel still running may need the columns to finish
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
     __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], o_free[2], ml_full;
@@ -168,7 +200,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     __shared__ volatile uint32_t fail;
     __shared__ uint32_t page_bits[TA_NOTES][WORDS];  // keys of a block whose page exists
     __shared__ unsigned long long broken[4];         // drafted values of a segment that are not finite
-    __shared__ float ml_s[128][2];
+    __shared__ float ml_s[128][2], copy_s[128][2], scale_s[128];
     __shared__ int64_t run_s[3];
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const PagedArgs& c = a.cache;
@@ -176,6 +208,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* k_s = q_s + T::QTILES * T::BOXES * T::Q_BOX;
     unsigned char* v_s = k_s + STAGES * T::BOXES * T::KV_BOX;
+    float* join_s = reinterpret_cast<float*>(v_s + STAGES * T::BOXES * T::KV_BOX);
 
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&ml_full, 4);
@@ -184,7 +217,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int i = 0; i < 4; ++i) broken[i] = 0;
         fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (const CUtensorMap* map : {&map_q, &map_k, &map_v}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
+    GLMB_PDL_PROLOGUE();  // before the TMEM allocation: a kernel still running may need the columns to finish
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -192,8 +227,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (warp == 9) {  // this CTA's run: equal numbers of blocks, in the order of the sequences
         auto blocks_of = [&](int b) {
             if (b >= c.seqs) return (int64_t)0;
-            const TreeSeq s = tree_seq(a, b, blockIdx.x == 0);
-            return (int64_t)s.blocks(KEYS) * sh.units(s.rows) * c.G;
+            return sh.share_of(tree_seq(a, b, blockIdx.x == 0), c.G);
         };
         int64_t mine = blocks_of(lane), total = mine;
         for (int b = lane + 32; b < c.seqs; b += 32) total += blocks_of(b);
@@ -228,7 +262,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     TreeWalk walk{run_s[0], 0, 0, 0};
     if (walk.left > 0) {
         walk.b = (int)run_s[1];
-        const int of = tree_seq(a, walk.b, false).blocks(KEYS);
+        const int of = sh.whole ? 1 : tree_seq(a, walk.b, false).blocks(KEYS);
         walk.at = (int)(run_s[2] / of), walk.block0 = (int)(run_s[2] % of);
     }
     // blocks of a segment that group t takes, and the n-th of them (counted from the segment's first)
@@ -486,69 +520,110 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (ok && both) ok = mbar_wait(o_full + 1, used[1] & 1) && mbar_wait(&ml_full, joined & 1) && !fail;
             ++used[t];
             if (both) ++used[1], ++joined;
-            if (!ok) break;
+            if (!ok) fail = 1;
+            if (!ok && !JOINS) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t lost = broken[segment & 3] & mask;
-            const bool whole = COPIES == 1 && s.blocks == s.of;  // nobody else has keys of this row
-            if (warp_live) {
-                float f0 = 1.f, f1 = 0.f;
-                if (both) {
-                    const float m1 = ml_s[row][0], l1 = ml_s[row][1], next = fmaxf(m, m1);
-                    f0 = m == next ? 1.f : ta_exp2(m - next);
-                    f1 = m1 == next ? 1.f : ta_exp2(m1 - next);
-                    l = l * f0 + l1 * f1;
-                    m = isnan(m1) ? m1 : next;
-                }
-                const int head = s.g * sh.per + hh, out_row = s.seq.row0 + j;
-                float scale = 1.f;
-                if (whole) {
-                    if (a.sink && live && a.sink[head] != -INFINITY) {
-                        const float sink2 = a.sink[head] * TA_LOG2E, next = fmaxf(m, sink2), f = m == -INFINITY ? 0.f : ta_exp2(m - next);
-                        scale = f / (l * f + ta_exp2(sink2 - next));
-                    } else {
-                        scale = l == 0.f ? 0.f : 1.f / l;
-                    }
-                }
-                bf16* dst = a.out + (int64_t)out_row * a.out_row + (int64_t)head * a.out_head;
-                const int64_t slot = ((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x;
-                const int64_t part = sh.part(slot, MODE == TA_PAIR ? t : 0, copy) + in;
-                for (int x0 = 0; x0 < c.vdim; x0 += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(tmem + 256 + t * 128 + lanes + x0, o);
-                    float y[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(o[i]);
-                    if (both) {
-                        tmem_ld16(tmem + 384 + lanes + x0, o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = y[i] * f0 + __uint_as_float(o[i]) * f1;
-                    }
-                    if (!live) continue;
-                    for (uint64_t left = lost; left; left &= left - 1) {  // drafted values that were left out of the product
-                        const int drafted_slot = s.seq.length + __ffsll(left) - 1, page = paged_page(c, s.b, drafted_slot);
-                        if (drafted_slot % KEYS / T::COLS != copy) continue;
-                        const bf16* k = c.k + page * c.k_page + (drafted_slot % c.page) * c.k_slot + s.g * c.k_head;
-                        const bf16* v = c.v + page * c.v_page + (drafted_slot % c.page) * c.v_slot + s.g * c.v_head + x0;
-                        const bf16* q = a.q + (int64_t)out_row * a.q_row + (int64_t)head * a.q_head;
-                        float dot = 0.f;
-                        for (int d = 0; d < c.dim; ++d) dot = fmaf(to_f32(q[d]), to_f32(k[d]), dot);
-                        const float p = ta_exp2(fmaf(dot, scale2, -m));
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = fmaf(p, to_f32(v[i]), y[i]);
-                    }
-                    if (whole) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = pack_bf16(y[2 * i] * scale, y[2 * i + 1] * scale);
-                        *reinterpret_cast<uint4*>(dst + x0) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(dst + x0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(a.part_o + part * c.vdim + x0 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-                    }
-                }
-                if (live && !whole) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m, l);
+            const bool whole = (JOINS || COPIES == 1) && s.blocks == s.of;  // nobody else has keys of this row
+            float f0 = 1.f, f1 = 0.f;
+            if (both) {
+                const float m1 = ml_s[row][0], l1 = ml_s[row][1], next = fmaxf(m, m1);
+                f0 = m == next ? 1.f : ta_exp2(m - next);
+                f1 = m1 == next ? 1.f : ta_exp2(m1 - next);
+                l = l * f0 + l1 * f1;
+                m = isnan(m1) ? m1 : next;
             }
+            const int head = s.g * sh.per + hh, out_row = s.seq.row0 + j;
+            const int64_t part = sh.part(((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x, MODE == TA_PAIR ? t : 0, JOINS ? 0 : copy);
+            if constexpr (JOINS) {  // every copy learns the sums of the row's keys
+                copy_s[row][0] = m, copy_s[row][1] = l;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                float next = m, all = 0.f;
+#pragma unroll
+                for (int k = 0; k < COPIES; ++k) next = fmaxf(next, copy_s[k * T::ROWS + in][0]);
+#pragma unroll
+                for (int k = 0; k < COPIES; ++k) {
+                    const float mk = copy_s[k * T::ROWS + in][0], lk = copy_s[k * T::ROWS + in][1];
+                    all += mk == next ? lk : lk * ta_exp2(mk - next);
+                }
+                const float f = m == next ? 1.f : ta_exp2(m - next);
+                f0 *= f, f1 *= f, m = next, l = all;
+            }
+            float scale = 1.f;
+            if (whole) {
+                const float sink2 = a.sink && live ? a.sink[head] * TA_LOG2E : -INFINITY;
+                if (sink2 != -INFINITY) {
+                    const float next = fmaxf(m, sink2), f = m == -INFINITY ? 0.f : ta_exp2(m - next);
+                    scale = f / (l * f + ta_exp2(sink2 - next));
+                } else {
+                    scale = l == 0.f ? 0.f : 1.f / l;
+                }
+            }
+            if (live && !whole) *reinterpret_cast<float2*>(a.part_ml + (part + in) * 2) = make_float2(m, l);
+            if (JOINS && copy == 0) scale_s[in] = scale;
+            for (int x1 = 0; x1 < c.vdim; x1 += 64) {
+                const int upto = min(c.vdim, x1 + 64);
+                if (warp_live)
+                    for (int x0 = x1; x0 < upto; x0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(tmem + 256 + t * 128 + lanes + x0, o);
+                        float y[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(o[i]) * f0;
+                        if (both) {
+                            tmem_ld16(tmem + 384 + lanes + x0, o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = fmaf(__uint_as_float(o[i]), f1, y[i]);
+                        }
+                        if (!live) continue;
+                        for (uint64_t left = lost; left; left &= left - 1) {  // drafted values that were left out of the product
+                            const int drafted_slot = s.seq.length + __ffsll(left) - 1, page = paged_page(c, s.b, drafted_slot);
+                            if (drafted_slot % KEYS / T::COLS != copy) continue;
+                            const bf16* k = c.k + page * c.k_page + (drafted_slot % c.page) * c.k_slot + s.g * c.k_head;
+                            const bf16* v = c.v + page * c.v_page + (drafted_slot % c.page) * c.v_slot + s.g * c.v_head + x0;
+                            const bf16* q = a.q + (int64_t)out_row * a.q_row + (int64_t)head * a.q_head;
+                            float dot = 0.f;
+                            for (int d = 0; d < c.dim; ++d) dot = fmaf(to_f32(q[d]), to_f32(k[d]), dot);
+                            const float p = ta_exp2(fmaf(dot, scale2, -m));
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = fmaf(p, to_f32(v[i]), y[i]);
+                        }
+                        if (JOINS) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(join_s + row * TA_JOIN + x0 - x1 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                        } else if (whole) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(y[2 * i] * scale, y[2 * i + 1] * scale);
+                            bf16* dst = a.out + (int64_t)out_row * a.out_row + (int64_t)head * a.out_head;
+                            *reinterpret_cast<uint4*>(dst + x0) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + x0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(a.part_o + (part + in) * c.vdim + x0 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                        }
+                    }
+                if constexpr (JOINS) {
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    const int pieces = (upto - x1) >> 2;  // of four columns
+                    for (int i = row; i < sh.heads * sh.tile_rows * pieces; i += 128) {
+                        const int r = i / pieces, d = i % pieces * 4, jr = j0 + r / sh.heads, hr = h0 + r % sh.heads;
+                        if (jr >= s.seq.rows || hr >= sh.per) continue;
+                        float4 y = *reinterpret_cast<const float4*>(join_s + r * TA_JOIN + d);
+#pragma unroll
+                        for (int k = 1; k < COPIES; ++k) {
+                            const float4 z = *reinterpret_cast<const float4*>(join_s + (k * T::ROWS + r) * TA_JOIN + d);
+                            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                        }
+                        const float f = scale_s[r];
+                        *reinterpret_cast<uint2*>(a.out + (int64_t)(s.seq.row0 + jr) * a.out_row + (int64_t)(s.g * sh.per + hr) * a.out_head + x1 + d) =
+                            make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+                    }
+                    if (upto < c.vdim) asm volatile("bar.sync 1, 128;" ::: "memory");  // before the next columns
+                }
+            }
+            if (JOINS && fail) ok = false;  // all four warps came to the same barriers
+            if (!ok) break;
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
@@ -560,6 +635,13 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             fail = 1;
             if (lane == 0) raise_status(a.status, GLMB_STATUS_WAIT_TIMEOUT);
         }
+        if (sh.whole && a.clear_rest)  // there is no second launch
+            for (int r = blockIdx.x * 8 + warp; r < a.rows; r += gridDim.x * 8) {
+                const TreeRow of = tree_row(a, sh, r, lane);
+                if (!of.mine)
+                    for (int i = lane; i < a.H * (c.vdim >> 3); i += 32)
+                        *reinterpret_cast<uint4*>(a.out + (int64_t)r * a.out_row + (int64_t)(i / (c.vdim >> 3)) * a.out_head + i % (c.vdim >> 3) * 8) = make_uint4(0, 0, 0, 0);
+            }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -569,93 +651,63 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
 }
 
-// A warp a row and head: joins the sums that several runs or copies left, or clears the row where it belongs to no sequence.  grid (rows, blocks of heads).
-__global__ void __launch_bounds__(TM_WARPS * 32) tree_merge_kernel(const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh) {
+// Joins the sums that several runs or copies left of a row's heads, or clears the row where it belongs to no sequence.  A warp a head, sixteen sums and their
+// scales on their way at once: with few rows its latency is its cost, with many the search for the row's sequence, which a CTA does once for its heads.
+// grid (rows, parts of the heads).
+__global__ void __launch_bounds__(256, 2) tree_merge_kernel(const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh) {
     GLMB_PDL_PROLOGUE();
+    constexpr int BATCH = 16;
     const PagedArgs& c = a.cache;
-    const int row = blockIdx.x, h = blockIdx.y * TM_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (h >= a.H) return;
-    // the row's sequence is the last that begins at or before it; blocks of all sequences, and of those that begin no later
-    int64_t total = 0, upto = 0;
-    int b = -1;
-    for (int b0 = 0; b0 < c.seqs; b0 += 32) {
-        bool begun = false;
-        if (b0 + lane < c.seqs) {
-            const TreeSeq s = tree_seq(a, b0 + lane, false);
-            const int64_t mine = (int64_t)s.blocks(sh.keys) * sh.units(s.rows) * c.G;
-            begun = a.starts[b0 + lane] <= row;
-            total += mine;
-            upto += begun ? mine : 0;
-        }
-        b += __popc(__ballot_sync(0xffffffffu, begun));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        upto += __shfl_xor_sync(0xffffffffu, upto, o);
-    }
-    bf16* dst = a.out + (int64_t)row * a.out_row + (int64_t)h * a.out_head;
-    TreeSeq seq{0, 0, 0, 0};
-    if (b >= 0) seq = tree_seq(a, b, false);
-    const int j = row - seq.row0;
-    if (b < 0 || j < 0 || j >= seq.rows) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x, h0 = blockIdx.y * 8 + (threadIdx.x >> 5), step = gridDim.y * 8;
+    const TreeRow of = tree_row(a, sh, row, lane);
+    bf16* dst = a.out + (int64_t)row * a.out_row;
+    if (!of.mine) {
         if (a.clear_rest)
-            for (int d = lane * 8; d < c.vdim; d += 256) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+            for (int h = h0; h < a.H; h += step)
+                for (int d = lane * 8; d < c.vdim; d += 256) *reinterpret_cast<uint4*>(dst + (int64_t)h * a.out_head + d) = make_uint4(0, 0, 0, 0);
         return;
     }
-    const int64_t share = (total + sh.ctas - 1) / sh.ctas;
-    const int blocks = seq.blocks(sh.keys), units = sh.units(seq.rows), g = h / sh.per, hh = h % sh.per;
-    const int tile = j / sh.tile_rows * sh.head_blocks + hh / sh.heads, unit = tile / sh.in_unit;
-    const int64_t from = upto - (int64_t)blocks * units * c.G + ((int64_t)g * units + unit) * blocks;
-    const int first = (int)(from / share), last = (int)((from + blocks - 1) / share), parts = (last - first + 1) * sh.copies;  // CTAs with keys of the unit
-    if (parts == 1) return;  // written already
-    const int64_t slot = ((int64_t)b * c.G + g) * sh.units_max + unit + first;
-    const int in = j % sh.tile_rows * sh.heads + hh % sh.heads;
-    auto place = [&](int k) { return sh.part(slot + k / sh.copies, tile % sh.in_unit, k % sh.copies) + in; };
-    float m = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;  // the same in every lane
-    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // columns 4 lane .. and 128 + 4 lane ..
-    const int d0 = lane * 4, d1 = 128 + lane * 4;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (k0 + lane < parts) ml = *reinterpret_cast<const float2*>(a.part_ml + place(k0 + lane) * 2);
-        const bool empty = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing there
-        const float next = fmaxf(m, warp_max(ml.x)), fix = m == next ? 1.f : ta_exp2(m - next);
-        const float w = empty ? 0.f : ml.x == next ? 1.f : ta_exp2(ml.x - next);
-        m = next;
-        l = l * fix + warp_sum(empty ? 0.f : ml.y * w);
+    const int64_t share = (of.total + sh.ctas - 1) / sh.ctas;
+    const int j = of.j, blocks = of.seq.blocks(sh.keys), units = sh.units(of.seq.rows), row_block = j / sh.tile_rows * sh.head_blocks;
+    const int rows_of = sh.heads * sh.tile_rows, segment = sh.in_unit * sh.copies * rows_of, shift = sh.copies == 4 ? 2 : sh.copies - 1;
+    auto offset = [&](int k) { return (k >> shift) * segment + (k & (sh.copies - 1)) * rows_of; };  // places of the k-th sum behind the first
+    for (int h = h0; h < a.H; h += step) {
+        const int g = h / sh.per, hh = h % sh.per, tile = row_block + hh / sh.heads, unit = tile / sh.in_unit;
+        const int64_t from = of.upto - (int64_t)blocks * units * c.G + ((int64_t)g * units + unit) * blocks;
+        const int first = (int)(from / share), last = (int)((from + blocks - 1) / share), parts = (last - first + 1) * sh.copies;  // CTAs with keys of the unit
+        if (parts == 1) continue;  // written already
+        const int64_t place = sh.part(((int64_t)of.b * c.G + g) * sh.units_max + unit + first, tile % sh.in_unit, 0) + j % sh.tile_rows * sh.heads + hh % sh.heads;
+        const float* part_ml = a.part_ml + place * 2;
+        const float* part_o = a.part_o + place * c.vdim;
+#pragma unroll 1
+        for (int d = lane * 4; d - lane * 4 < c.vdim; d += 128) {
+            float m = a.sink ? a.sink[h] * TA_LOG2E : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;  // the same in every lane
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int k0 = 0; k0 < parts; k0 += BATCH) {
+                float4 v[BATCH];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= fix;
-        const int here = min(32, parts - k0);
-        const int64_t at = k0 + lane < parts ? place(k0 + lane) * c.vdim : 0;
-        for (int k = 0; k < here; k += 8) {  // eight on their way; an empty sum is zeros
-            float4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int64_t from_k = __shfl_sync(0xffffffffu, at, k + u);
-                v[u] = k + u < here && d0 < c.vdim ? *reinterpret_cast<const float4*>(a.part_o + from_k + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float wk = __shfl_sync(0xffffffffu, w, k + u);
-                o[0] = fmaf(wk, v[u].x, o[0]), o[1] = fmaf(wk, v[u].y, o[1]), o[2] = fmaf(wk, v[u].z, o[2]), o[3] = fmaf(wk, v[u].w, o[3]);
-            }
-            if (c.vdim > 128) {
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int64_t from_k = __shfl_sync(0xffffffffu, at, k + u);
-                    v[u] = k + u < here && d1 < c.vdim ? *reinterpret_cast<const float4*>(a.part_o + from_k + d1) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < BATCH; ++u) {
+                    v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (k0 + u < parts && d < c.vdim) v[u] = *reinterpret_cast<const float4*>(part_o + offset(k0 + u) * c.vdim + d);
                 }
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (lane < BATCH && k0 + lane < parts) ml = *reinterpret_cast<const float2*>(part_ml + offset(k0 + lane) * 2);
+                const float next = fmaxf(m, warp_max(ml.x)), fix = m == next ? 1.f : ta_exp2(m - next);
+                const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.x == next ? 1.f : ta_exp2(ml.x - next);  // saw nothing there: zeros
+                m = next;
+                l = l * fix + warp_sum(w == 0.f ? 0.f : ml.y * w);
+                o = make_float4(o.x * fix, o.y * fix, o.z * fix, o.w * fix);
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const float wk = __shfl_sync(0xffffffffu, w, k + u);
-                    o[4] = fmaf(wk, v[u].x, o[4]), o[5] = fmaf(wk, v[u].y, o[5]), o[6] = fmaf(wk, v[u].z, o[6]), o[7] = fmaf(wk, v[u].w, o[7]);
+                for (int u = 0; u < BATCH; ++u) {
+                    const float wu = __shfl_sync(0xffffffffu, w, u);
+                    o.x = fmaf(wu, v[u].x, o.x), o.y = fmaf(wu, v[u].y, o.y), o.z = fmaf(wu, v[u].z, o.z), o.w = fmaf(wu, v[u].w, o.w);
                 }
             }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (d < c.vdim) *reinterpret_cast<uint2*>(dst + (int64_t)h * a.out_head + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d0 < c.vdim) *reinterpret_cast<uint2*>(dst + d0) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-    if (d1 < c.vdim) *reinterpret_cast<uint2*>(dst + d1) = make_uint2(pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
@@ -668,16 +720,18 @@ static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
     const int tiles = ceil_div(a.max_rows, sh.tile_rows) * sh.head_blocks;
     mode = a.cache.dim > 128 || a.cache.vdim > 128 ? TA_WIDE : tiles > 1 ? TA_PAIR : TA_SINGLE;
     sh.in_unit = mode == TA_PAIR ? 2 : 1;
-    const int tile = sh.heads * sh.tile_rows;
-    sh.copies = mode == TA_PAIR || tile > 64 ? 1 : tile > 32 || mode == TA_WIDE ? 2 : 4;
     sh.keys = mode == TA_WIDE ? 64 : 128;
     sh.ctas = 148;
     sh.units_max = ceil_div(tiles, sh.in_unit);
+    const int tile = sh.heads * sh.tile_rows;
+    sh.copies = mode == TA_PAIR || tile > 64 ? 1 : tile > 32 || mode == TA_WIDE ? 2 : 4;
+    sh.whole = (int64_t)a.cache.per_seq * a.cache.page <= TA_WHOLE_BLOCKS * sh.keys;
+    if (sh.whole && mode == TA_WIDE) sh.copies = 1;  // no room to join copies in
     return sh;
 }
 // Sums that all segments may leave: one for each unit and one more for each CTA.
 static int64_t tree_parts(const TreeAttentionArgs& a, const TreeShape& sh) {
-    return ((int64_t)a.cache.seqs * a.cache.G * sh.units_max + sh.ctas) * sh.in_unit * sh.copies * sh.heads * sh.tile_rows;
+    return sh.whole ? 0 : ((int64_t)a.cache.seqs * a.cache.G * sh.units_max + sh.ctas) * sh.in_unit * sh.copies * sh.heads * sh.tile_rows;
 }
 static int tree_refuses(const TreeAttentionArgs& a) {
     const PagedArgs& c = a.cache;
@@ -704,9 +758,9 @@ static int tree_query_map(CUtensorMap* map, const TreeAttentionArgs& a, const Tr
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
 }
 
-template <int MODE, int COPIES>
+template <int MODE, int COPIES, bool JOINS>
 static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStream_t stream) {
-    typedef TreeMode<MODE, COPIES> T;
+    typedef TreeMode<MODE, COPIES, JOINS> T;
     int chunk = 8;  // slots that lie in one page wherever a block begins
     while (chunk < T::KEYS && a.cache.page % (2 * chunk) == 0) chunk *= 2;
     const PagedArgs& c = a.cache;
@@ -718,14 +772,15 @@ static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStre
     static DeviceOnce once;
     const int dev = once.pending();
     if (dev != DeviceOnce::SET) {
-        const cudaError_t e = cudaFuncSetAttribute((const void*)tree_attention_kernel<MODE, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute((const void*)tree_attention_kernel<MODE, COPIES, JOINS>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
         if (e != cudaSuccess) return (int)e;
         once.mark(dev);
     }
-    GLMB_LAUNCH((tree_attention_kernel<MODE, COPIES>), sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
+    GLMB_LAUNCH((tree_attention_kernel<MODE, COPIES, JOINS>), sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
     const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return (int)e;
-    GLMB_LAUNCH(tree_merge_kernel, dim3(a.rows, ceil_div(a.H, TM_WARPS)), TM_WARPS * 32, 0, stream, a, sh);
+    if (e != cudaSuccess || sh.whole) return (int)e;
+    const int heads_at_once = min(ceil_div(a.H, 8), ceil_div(148 * 2, a.rows));
+    GLMB_LAUNCH(tree_merge_kernel, dim3(a.rows, heads_at_once), 256, 0, stream, a, sh);
     return (int)cudaGetLastError();
 }
 
@@ -745,8 +800,10 @@ GLMB_API int glmb_tree_attention(const TreeAttentionArgs* args, cudaStream_t str
     if (a.cache.seqs == 0 || a.rows == 0) return 0;
     int mode;
     const TreeShape sh = tree_shape(a, mode);
-    if (a.parts < tree_parts(a, sh) || !a.part_o || !a.part_ml) return 1;
-    if (mode == TA_PAIR) return tree_launch<TA_PAIR, 1>(a, sh, stream);
-    if (mode == TA_WIDE) return sh.copies == 1 ? tree_launch<TA_WIDE, 1>(a, sh, stream) : tree_launch<TA_WIDE, 2>(a, sh, stream);
-    return sh.copies == 1 ? tree_launch<TA_SINGLE, 1>(a, sh, stream) : sh.copies == 2 ? tree_launch<TA_SINGLE, 2>(a, sh, stream) : tree_launch<TA_SINGLE, 4>(a, sh, stream);
+    if (a.parts < tree_parts(a, sh) || (!sh.whole && (!a.part_o || !a.part_ml))) return 1;
+    if (mode == TA_PAIR) return tree_launch<TA_PAIR, 1, false>(a, sh, stream);
+    if (mode == TA_WIDE) return sh.copies == 1 ? tree_launch<TA_WIDE, 1, false>(a, sh, stream) : tree_launch<TA_WIDE, 2, false>(a, sh, stream);
+    if (sh.copies == 1) return tree_launch<TA_SINGLE, 1, false>(a, sh, stream);
+    if (sh.copies == 2) return sh.whole ? tree_launch<TA_SINGLE, 2, true>(a, sh, stream) : tree_launch<TA_SINGLE, 2, false>(a, sh, stream);
+    return sh.whole ? tree_launch<TA_SINGLE, 4, true>(a, sh, stream) : tree_launch<TA_SINGLE, 4, false>(a, sh, stream);
 }

@@ -970,9 +970,10 @@ def tree_attention(q, cache: PagedArgs, starts, lengths, masks, scale, max_rows,
     parts = _lib.glmb_tree_attention_parts(C.byref(a))  # not a launch: past the wrapper that times launches
     if parts < 0:
         raise ValueError("tree_attention: sizes that the kernels do not take")
-    room = torch.empty(parts * (cache.vdim + 2), dtype=torch.float32, device=q.device)  # sums of keys that several CTAs share
-    a.part_o = room.data_ptr()
-    a.part_ml, a.parts = a.part_o + 4 * parts * cache.vdim, parts
+    if parts:  # sums of keys that several CTAs share
+        room = torch.empty(parts * (cache.vdim + 2), dtype=torch.float32, device=q.device)
+        a.part_o = room.data_ptr()
+        a.part_ml, a.parts = a.part_o + 4 * parts * cache.vdim, parts
     _check(launch(C.byref(a), _stream()), "tree_attention")
 
 
