@@ -23,9 +23,10 @@ OBJ_DIR = CSRC / "build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 # sources each model family needs when the complete library has not been built
 COMPONENTS = {
-    "namizen": ("parallel_block", "qkv_conv", "chunk_attention", "chunk_attention_tcgen05", "gemm_f32", "swiglu_rows", "gemv", "gemm_tcgen05", "misc", "peer_registry"),
+    "namizen": ("parallel_block", "qkv_conv", "chunk_attention", "chunk_attention_tcgen05", "gemm_f32", "swiglu_rows", "gemv", "gemm_tcgen05", "misc", "peer_registry",
+                "logprobs", "head_logprobs_tcgen05"),
     "zikevik": ("parallel_block", "delta_rule", "delta_chunk", "delta_step", "latent", "latent_decode", "chunk_attention", "chunk_attention_tcgen05", "moe_rows", "route_sort", "gemm_f32", "swiglu_rows",
-                "gemv", "gemm_tcgen05", "misc", "peer_registry"),
+                "gemv", "gemm_tcgen05", "misc", "peer_registry", "logprobs", "head_logprobs_tcgen05"),
 }
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -9,6 +9,12 @@ are over after the step (their lane is given back).  The logits of a step go to 
 in the order of the entries and of ``want``; a step in which nothing is wanted writes no file.  After every step a line ``done <step>``
 is printed.
 
+An entry with ``"score"`` instead of ``want`` has its tokens scored: ``{"id": "a", "tokens": [5, 17, 3], "score": {"top": 2, "next": 9}}`` asks at every
+place for the log probability of the token that comes after it (``next``, which may be left out, after the last) and for the ``top`` most likely ones
+(0 to 32; left out: none).  The scores of a step go to ``<out>/<step>.scores.json``, a list with an object for every scored entry: ``id``,
+``logprob``, ``entropy`` and ``best`` (the most likely token's log probability), a number a place (null: nothing was asked there, or the place has no probabilities), and
+``top``, ``[token, log probability]`` pairs a place.  Natural logarithms; minus infinity is written as -Infinity.
+
 The requests run on the engine's own lanes: a request's later single tokens go through the decode program's kernels (those of one step
 together, one lane each), everything else through the prefill program, both from the cache that earlier steps left.
 
@@ -18,6 +24,7 @@ Exit status 3: the model has no path in the asked-for number format.
 from __future__ import annotations
 
 import json
+import math
 import sys
 from pathlib import Path
 
@@ -27,11 +34,30 @@ LANES = 4
 PREFILL_CHUNK = 2048
 
 
+def _check_score(entry: dict) -> None:
+    asked = entry["score"]
+    if not isinstance(asked, dict) or set(asked) - {"top", "next"} or entry.get("want"):
+        raise RequestValidationError("an entry is scored with top and next, and has no wanted places then")
+    top, following = asked.get("top", 0), asked.get("next", 0)
+    if type(top) is not int or not 0 <= top <= 32 or type(following) is not int or following < 0:
+        raise RequestValidationError("top is between 0 and 32, next a token id")
+
+
+def _scores_of(name: str, scores) -> dict:
+    numbers = lambda values: [None if math.isnan(v) else v for v in values.tolist()]  # noqa: E731
+    out = {"id": name, "logprob": numbers(scores.logprob), "entropy": numbers(scores.entropy), "best": numbers(scores.best)}
+    if scores.top_ids is not None:
+        out["top"] = [list(map(list, zip(ids, numbers(values)))) for ids, values in zip(scores.top_ids.tolist(), scores.top_logprobs)]
+    return out
+
+
 class TraceReplay:
-    """Requests by name on the lanes of a runner.  The runner needs ``lanes``, ``lengths``, ``open_lane``, ``extend`` and ``decode_logits``."""
+    """Requests by name on the lanes of a runner.  The runner needs ``lanes``, ``lengths``, ``open_lane``, ``extend`` and ``decode_logits``, and ``score``
+    for entries that are scored."""
 
     def __init__(self, runner):
         self.runner = runner
+        self.scores: list[dict] = []  # of the last step
         self.free = list(range(runner.lanes))
         self.lane_of: dict[str, int] = {}
 
@@ -49,12 +75,19 @@ class TraceReplay:
         names = [e["id"] for e in entries]
         if len(set(names)) != len(names):
             raise RequestValidationError("a request has two entries in one step")
+        for entry in entries:
+            if "score" in entry:
+                _check_score(entry)
+        self.scores = []
         lanes = [self._lane(name) for name in names]
-        single = {lane: e["tokens"][0] for lane, e in zip(lanes, entries) if len(e["tokens"]) == 1 and self.runner.lengths[lane] > 0}
+        single = {lane: e["tokens"][0] for lane, e in zip(lanes, entries) if len(e["tokens"]) == 1 and self.runner.lengths[lane] > 0 and "score" not in e}
         decoded = self.runner.decode_logits(single) if single else {}
         rows = []
         for lane, entry in zip(lanes, entries):
-            if lane in decoded:
+            if "score" in entry:
+                asked = entry["score"]
+                self.scores.append(_scores_of(entry["id"], self.runner.score(lane, entry["tokens"], following=asked.get("next"), top=asked.get("top", 0))))
+            elif lane in decoded:
                 rows += [decoded[lane] for _ in entry["want"]]
             else:
                 rows += list(self.runner.extend(lane, entry["tokens"], entry["want"]))
@@ -78,6 +111,8 @@ def replay(runner, lines, out: Path, emit=print) -> None:
         rows = session.step(command)
         if rows:
             write_rows(out / f"{int(command['step'])}.f32", rows)
+        if session.scores:
+            (out / f"{int(command['step'])}.scores.json").write_text(json.dumps(session.scores) + "\n")
         emit(f"done {int(command['step'])}", flush=True)
 
 

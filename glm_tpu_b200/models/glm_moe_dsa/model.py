@@ -715,7 +715,8 @@ class GlmMoeDsaModel:
 
         ``head='logits'`` returns the bf16 logits of ``head_rows`` (this rank's vocabulary slice).  ``head='argmax'``
         (decode) fuses the greedy reduction into the lm_head kernel: the packed best candidate of every row lands in
-        ``ws.local_best`` and ``None`` is returned; ``sample`` then finishes the step.
+        ``ws.local_best`` and ``None`` is returned; ``sample`` then finishes the step.  ``head='hidden'`` returns what the
+        vocabulary is multiplied with (a view of the workspace).
         """
         g = self.g
         native.embed_rows(tokens, self.w.embed, ws.residual, self.peer.status_ptr)
@@ -738,6 +739,8 @@ class GlmMoeDsaModel:
         hs = slice(0, rows) if head_rows is None else head_rows  # a slice, or an index tensor
         xh = ws.x[hs]
         n = xh.shape[0]
+        if head == "hidden":
+            return xh
         if head == "argmax":
             native.skinny_bf16(xh, self.w.lm_head, ws.local_best, native.SK_OUT_ARGMAX, comm=self.peer.comm,
                                channel=self.rank * self.layout.vocab_local, os_=0)
@@ -747,6 +750,14 @@ class GlmMoeDsaModel:
         else:
             self._mm(xh, self.w.lm_head, out=ws.logits[:n])
         return ws.logits[:n]
+
+    @property
+    def head_table(self) -> torch.Tensor:
+        return self.w.lm_head
+
+    def head_logits(self, x: torch.Tensor) -> torch.Tensor:
+        """The fp32 logits of hidden rows (``head='hidden'``), not rounded to bf16 as a decoding step's are."""
+        return self._mm(x, self.w.lm_head, f32=True)
 
     def sample(self, ws: Workspace, state: DecoderState, logits: torch.Tensor, rows: int, row_active, *, advance: int,
                tokens_out=None, positions=None, out=None) -> None:

@@ -197,7 +197,8 @@ class NamizenModel:
         """Push ``rows`` token rows through the decoder; in prefill they are the positions ``max_ctx - rows .. max_ctx - 1`` of one lane.
 
         ``head='logits'`` returns the fp32 logits of ``head_rows`` (a slice or an index tensor; ``None``: all rows); ``head='argmax'``
-        (decode) leaves the packed best candidates in ``ws.local_best`` and returns ``None``; ``head='none'`` stops after the layers.
+        (decode) leaves the packed best candidates in ``ws.local_best`` and returns ``None``; ``head='none'`` stops after the layers;
+        ``head='hidden'`` returns what the vocabulary is multiplied with (a view of the workspace).
         """
         g, w, eps = self.g, self.w, self.g.norm_eps
         start = 0 if decode else max_ctx - rows
@@ -216,12 +217,24 @@ class NamizenModel:
             return None
         native.parallel_norm(residual, g.hidden_size, w.final_norm, ws.h1[:rows], eps, update=update, status=self.peer.status_ptr)
         x = ws.h1[:rows] if head_rows is None else ws.h1[:rows][head_rows]
+        if head == "hidden":
+            return x
         if head == "argmax" and not self.is_f32:
             native.skinny_bf16(x, w.head, ws.local_best, native.SK_OUT_ARGMAX_F32, N=g.vocab_size, comm=self.peer.comm, channel=0, os_=0)
             return None
         logits = ws.logits if decode else torch.empty((x.shape[0], w.head.shape[0]), dtype=torch.float32, device=self.device)
         self._mm(x, w.head, logits[: x.shape[0]])
         return logits[: x.shape[0], : g.vocab_size]
+
+    @property
+    def head_table(self) -> torch.Tensor:
+        return self.w.head
+
+    def head_logits(self, x: torch.Tensor) -> torch.Tensor:
+        """The fp32 logits of hidden rows (``head='hidden'``)."""
+        logits = torch.empty((x.shape[0], self.w.head.shape[0]), dtype=torch.float32, device=self.device)
+        self._mm(x, self.w.head, logits)
+        return logits[:, : self.g.vocab_size]
 
     def sample(self, ws: NamizenWorkspace, state: RingState, logits, rows: int, row_active, *, advance: int, tokens_out=None, positions=None,
                out=None) -> None:

@@ -20,8 +20,12 @@ from dataclasses import dataclass, field
 
 import torch
 
+from glm_tpu_b200.exceptions import DeviceStatusError, PlanValidationError
 from glm_tpu_b200.runner.admission import check_collective_plan
 from glm_tpu_b200.runner.lane_state import RING
+
+
+SCORED_ROWS = 256  # rows of logits that scoring with alternatives keeps at once
 
 
 @dataclass
@@ -194,9 +198,9 @@ class LaneRunner:
                 self.prefill_ws = self._prefill_workspace()
         return self.prefill_ws
 
-    def _chunks(self, lane: int, token_ids, first: int, head_rows):
+    def _chunks(self, lane: int, token_ids, first: int, head_rows, head: str = "logits"):
         """Push ``token_ids`` through ``lane`` from position ``first`` on, ``prefill_chunk`` rows at a time.  ``head_rows(start, rows)``
-        names the rows of a chunk (counted from ``first``) whose logits are computed; yields ``(start, logits)`` per chunk."""
+        names the rows of a chunk (counted from ``first``) whose logits (``head``) are computed; yields ``(start, logits)`` per chunk."""
         n = len(token_ids)
         ws, st, m = self._ensure_prefill_ws(), self.state, self.model
         ids = _host_ids(token_ids).pin_memory().to(self.device, non_blocking=True)
@@ -205,7 +209,7 @@ class LaneRunner:
             rows = min(self.prefill_chunk, n - start)
             pos = torch.arange(first + start, first + start + rows, dtype=torch.int32, device=self.device)
             yield start, m.run_rows(ws, st, ids[start : start + rows], pos, lane_t, None, rows, decode=False, max_ctx=first + start + rows,
-                                    head_rows=head_rows(start, rows), lane_of_rows=lane)
+                                    head_rows=head_rows(start, rows), head=head, lane_of_rows=lane)
 
     def prefill(self, lane: int, token_ids) -> int:
         """Run a prompt through ``lane`` with a fresh cache; returns the first generated token.
@@ -268,6 +272,41 @@ class LaneRunner:
             self.state.positions[lane].fill_(first + n)
             self.peer.check_status()
         return out if out is not None else torch.empty((0, self.g.vocab_size))
+
+    def score(self, lane: int, token_ids, *, following: int | None = None, top: int = 0):
+        """Run the next tokens of ``lane`` through the prefill program as ``extend`` does and score them: place ``i`` is asked for the token
+        at ``i + 1``, the last place for ``following`` (without one its log probability is NaN).  Returns ``TokenLogprobs`` on the CPU, with the
+        ``top`` most likely tokens of every place where asked for.  The logits are those of the family in fp32, not rounded, and are not kept."""
+        from glm_tpu_b200.layers import logprobs
+        from glm_tpu_b200.layers.contracts import TokenLogprobs
+
+        n, first = len(token_ids), self.lengths[lane]
+        if self.world > 1:
+            raise PlanValidationError("tokens are scored on one GPU: the vocabulary of this runner is split")
+        if not n or first + n > self.cache.context_capacity:
+            raise ValueError("the tokens do not fit the context capacity")
+        if not 0 <= top <= min(logprobs.MAX_TOP, self.g.vocab_size):
+            raise ValueError(f"between 0 and {min(logprobs.MAX_TOP, self.g.vocab_size)} alternatives")
+        parts = []
+        with torch.cuda.device(self.device):
+            asked = _host_ids([*list(token_ids)[1:], -1 if following is None else following]).pin_memory().to(self.device, non_blocking=True)
+            status = torch.zeros(1, dtype=torch.int32, device=self.device)
+            for start, hidden in self._chunks(lane, token_ids, first, lambda start, rows: slice(0, rows), head="hidden"):
+                step = SCORED_ROWS if top else hidden.shape[0]  # rows whose logits are in memory at once: none without alternatives
+                for r in range(0, hidden.shape[0], step):
+                    x, k = hidden[r : r + step], asked[start + r : start + min(r + step, hidden.shape[0])]
+                    if top:
+                        parts.append(logprobs.token_logprobs(self.model.head_logits(x), k, top=top, status=status))
+                    else:
+                        parts.append(logprobs.head_logprobs(x, self.model.head_table, k, vocab=self.g.vocab_size, status=status))
+            self.lengths[lane] = first + n
+            self.state.positions[lane].fill_(first + n)
+            scores = TokenLogprobs(*(torch.cat(column).cpu() if column[0] is not None else None for column in zip(*(vars(p).values() for p in parts))))
+            self.peer.check_status()
+            bits = int(status)
+            if bits:
+                raise DeviceStatusError("device status: a scored token lies outside the vocabulary, or a place has no finite logits", bits)
+        return scores
 
     def decode_logits(self, tokens: dict) -> dict:
         """One step of the decode program's kernels for the lanes of ``tokens`` (``lane -> its next token``; every other lane is frozen),
