@@ -9,7 +9,7 @@
 // sequence whose rows or length are out of range.
 //
 // A tile is up to 128 (drafted row, head) pairs of one key head: the M of both products.  A unit is a sequence's key head with one tile, or with two that
-// take turns on the tensor core; its keys come in blocks of 128.  The blocks of all units, one after another, are dealt to one CTA per SM in equal runs, so
+// take turns on the tensor core; its keys come in blocks of 128 or 64.  The blocks of all units, one after another, are dealt to one CTA per SM in equal runs, so
 // that unequal sequences keep every SM streaming; a run may begin and end inside a unit.  For each block of a tile:
 //
 //   S = Q K^T       both operands K-major in shared memory (TMA, 128-byte swizzle), fp32 scores in TMEM
@@ -20,13 +20,21 @@
 // are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs, or in shared memory.
 //
 // The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
-// (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-9 beside that of the result.
+// (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-8 each beside that of the result.  What
+// bounds them is one warp that issues for both: a block of 128 keys of two tiles takes 2.7 thousand cycles of softmax (2.0 of them exponentials) and 1.9 until
+// the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 4 heads at 131,000 slots: 296 us, 303 before
+// the softmax threads got the registers that their scores need (167 -> 157 for 4 x 64 drafts at 30,000).  Measured beside those 303: two buffers of scores, blocks
+// of 64 keys 424 us, with two issuing warps 303; blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
 // A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; memory is its bound, so its weights
-// keep a second piece, the remainder of the first.  Heads wider than 128 (WIDE): blocks of 64 keys, one group.
+// keep a second piece, the remainder of the first.  Heads wider than 128 (WIDE): blocks of 64 keys, one group, and two buffers of scores, so that the next ones are there
+// when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer 320).
 //
 //   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
 //   warp 8           issues every tcgen05.mma, owns the TMEM allocation
 //   warps 9, 10      look pages up, bring queries and keys, and values, in by TMA
+//
+// One warp issues for both groups and so waits for every block, in order: a warp that skipped the other group's blocks could take an older phase of a barrier
+// for the one it waits for.
 //
 // What a row does not see must not reach it, and a weight of zero times NaN is NaN.  Slots behind the last one, and pages that do not exist, are read as zeros
 // (out of the tensor map's range) or cleared in shared memory before the product; drafted values that are not finite are cleared too, and the rows
@@ -42,7 +50,6 @@
 
 #define TA_LOG2E 1.4426950408889634f
 #define TA_MAX_DRAFTS 64  // bits of a mask
-#define TA_THREADS 352
 #define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
 #define TA_JOIN 68        // floats of a row of joined sums: 64 columns, padded
 #define TA_WHOLE_BLOCKS 4 // caches of so few blocks a sequence: units are not split
@@ -179,23 +186,24 @@ __device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
 }
 
 template <int MODE, int COPIES, bool JOINS> struct TreeMode {
-    static constexpr int ROWS = 128 / COPIES, COLS = (MODE == TA_WIDE ? 64 : 128) / COPIES;  // rows of the tile, keys of a block that a thread weighs
-    static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2;
+    static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, ROWS = 128 / COPIES, COLS = KEYS / COPIES;  // rows of the tile, keys of a block that a thread weighs
+    static constexpr int GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2, SCORES = MODE == TA_WIDE ? 2 : 1;  // buffers
     static constexpr int STAGES = MODE == TA_SINGLE && !JOINS ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
+    static constexpr int THREADS = MODE == TA_PAIR ? 384 : 352;  // a pair's last warp is there to give its registers away
     static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
     static constexpr int JOIN = JOINS ? 128 * TA_JOIN * 4 : 0;  // 64 columns of the copies' sums
     static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + JOIN + 1024;
 };
 
 template <int MODE, int COPIES, bool JOINS>
-__global__ void __launch_bounds__(TA_THREADS, 1)
+__global__ void __launch_bounds__(TreeMode<MODE, COPIES, JOINS>::THREADS, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ TreeAttentionArgs a, const __grid_constant__ TreeShape sh, int slots_first_k, int slots_first_v, int chunk) {
     typedef TreeMode<MODE, COPIES, JOINS> T;
     constexpr int KEYS = T::KEYS, STAGES = T::STAGES, WORDS = KEYS / 32;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], o_free[2], ml_full;
+    __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], ml_full;  // of a group (and of its buffer of scores)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t fail;
     __shared__ uint32_t page_bits[TA_NOTES][WORDS];  // keys of a block whose page exists
@@ -212,7 +220,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&ml_full, 4);
-        for (int i = 0; i < 2; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1), mbar_init(o_free + i, 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(o_full + i, 1), mbar_init(o_free + i, 4), mbar_init(pv_done + i, 1);
+            for (int e = 0; e < 2; ++e) mbar_init(&s_full[i][e], 1), mbar_init(&p_full[i][e], 4);
+        }
         for (int i = 0; i < STAGES; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1), mbar_init(v_full + i, 1), mbar_init(v_empty + i, 1);
         for (int i = 0; i < 4; ++i) broken[i] = 0;
         fail = 0;
@@ -257,7 +268,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_slot;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 256 and 384
+    const uint32_t tmem = tmem_slot;  // scores of the groups at columns 0 and 128 (a second buffer 64 behind), O_0, O_1 at 256 and 384
 
     TreeWalk walk{run_s[0], 0, 0, 0};
     if (walk.left > 0) {
@@ -276,7 +287,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     TreeSegment s;
     uint32_t gone = 0;  // blocks of the segments before this one
     int segment = 0;
-    if (warp >= 9) {  // keys (and queries), values
+    if (MODE == TA_PAIR) {  // 384 x 168 registers at the launch: 256 x 200 and 128 x 104
+        if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    }
+    if (warp == 11) {  // of a pair
+    } else if (warp >= 9) {  // keys (and queries), values
         const bool keys = warp == 9;
         const int boxes = keys ? kboxes : vboxes, chunks = KEYS / chunk;
         const CUtensorMap* map = keys ? &map_k : &map_v;
@@ -334,50 +350,66 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
     } else if (warp == 8) {
         const uint32_t idesc_s = umma_idesc_bf16(128, KEYS), idesc_o = umma_idesc_bf16(128, c.vdim) | (1u << 16);  // bit 16: B is MN-major
-        uint32_t done[2] = {0, 0}, uses[2] = {0, 0};  // blocks and segments of a group so far
+        uint32_t made[2] = {0, 0}, done[2] = {0, 0}, uses[2] = {0, 0};  // blocks of scores, of outputs, and segments of a group so far
         bool ok = true;
         for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
             const int count[2] = {group_blocks(s, 0), group_blocks(s, 1)}, most = max(count[0], count[1]);
             if (!mbar_wait_warp(&q_full, segment & 1)) { fail = 1; break; }
+            auto last_of_block = [&](int t) { return MODE != TA_PAIR || t == 1 || count[1] == 0; };
+            auto scores = [&](int t, int j) {  // S_t = Q_t K^T
+                const uint32_t n = gone + nth(t, j), st = n % STAGES, buffer = T::SCORES == 2 ? made[t] & 1 : 0;
+                if (!mbar_wait_warp(k_full + st, (n / STAGES) & 1)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t q_at = umma_desc_sw128(smem_u32(q_s + (MODE == TA_PAIR ? t : 0) * kboxes * T::Q_BOX)), k_at = umma_desc_sw128(smem_u32(k_s + st * kboxes * T::KV_BOX));
+                const uint32_t s_at = tmem + t * 128 + buffer * 64;
+                if (elect_one()) {
+                    for (int x = 0; x < kboxes; ++x)  // a step of 16 columns: 32 bytes, 2 in the descriptor
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (x * 64 + k * 16 < c.dim)
+                                umma_bf16(s_at, q_at + x * (T::Q_BOX / 16) + k * 2, k_at + x * (T::KV_BOX / 16) + k * 2, idesc_s, (x > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&s_full[t][buffer]);
+                    if (last_of_block(t)) umma_commit(k_empty + st);
+                    if (nth(t, j) + 1 == s.blocks && last_of_block(t)) umma_commit(&q_empty);  // the segment's last scores
+                }
+                __syncwarp();
+                ++made[t];
+                return true;
+            };
+            auto outputs = [&](int t, int j) {  // O_t += P_t V
+                const uint32_t n = gone + nth(t, j), st = n % STAGES, buffer = T::SCORES == 2 ? done[t] & 1 : 0, use = T::SCORES == 2 ? done[t] >> 1 : done[t];
+                if (!((j > 0 || uses[t] == 0 || mbar_wait_warp(o_free + t, (uses[t] - 1) & 1)) && mbar_wait_warp(&p_full[t][buffer], use & 1) &&
+                      mbar_wait_warp(v_full + st, (n / STAGES) & 1)))
+                    return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t v_at = ta_desc_mn(smem_u32(v_s + st * vboxes * T::KV_BOX), T::KV_BOX);
+                const uint32_t p_addr = tmem + t * 128 + buffer * 64;
+                if (elect_one()) {
+#pragma unroll
+                    for (int piece = 0; piece < T::PIECES; ++piece)
+#pragma unroll
+                        for (int k = 0; k < KEYS / 16; ++k)
+                            umma_bf16_ts(tmem + 256 + t * 128, p_addr + piece * (KEYS / 2) + k * 8, v_at + k * 128, idesc_o, (j > 0 || piece > 0 || k > 0) ? 1u : 0u);
+                    if (T::SCORES == 2) umma_commit(pv_done + t);
+                    if (last_of_block(t)) umma_commit(v_empty + st);  // the values may be replaced once they have been read
+                    if (j + 1 == count[t]) umma_commit(o_full + t);
+                }
+                __syncwarp();
+                ++done[t];
+                if (j + 1 == count[t]) ++uses[t];
+                return true;
+            };
             for (int j = -1; j < most && ok; ++j) {
+                if (T::SCORES == 2) {  // the next scores are there before the softmax asks for them
 #pragma unroll
-                for (int t = 0; t < T::GROUPS; ++t) {
-                    if (ok && j >= 0 && j < count[t]) {  // O_t += P_t V
-                        const uint32_t n = gone + nth(t, j), st = n % STAGES;
-                        ok = (j > 0 || uses[t] == 0 || mbar_wait_warp(o_free + t, (uses[t] - 1) & 1)) && mbar_wait_warp(p_full + t, done[t] & 1) &&
-                             mbar_wait_warp(v_full + st, (n / STAGES) & 1);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t v_addr = smem_u32(v_s + st * vboxes * T::KV_BOX);
-                        if (elect_one()) {
+                    for (int t = 0; t < T::GROUPS; ++t) ok = ok && (j + 1 >= count[t] || scores(t, j + 1));
 #pragma unroll
-                            for (int piece = 0; piece < T::PIECES; ++piece)
+                    for (int t = 0; t < T::GROUPS; ++t) ok = ok && (j < 0 || j >= count[t] || outputs(t, j));
+                } else {
 #pragma unroll
-                                for (int k = 0; k < KEYS / 16; ++k)
-                                    umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + piece * (KEYS / 2) + k * 8, ta_desc_mn(v_addr + k * 2048, T::KV_BOX), idesc_o,
-                                                 (j > 0 || piece > 0 || k > 0) ? 1u : 0u);
-                            if (MODE != TA_PAIR || t == 1 || count[1] == 0) umma_commit(v_empty + st);  // the values may be replaced once they have been read
-                            if (j + 1 == count[t]) umma_commit(o_full + t);
-                        }
-                        __syncwarp();
-                        ++done[t];
-                        if (j + 1 == count[t]) ++uses[t];
-                    }
-                    if (ok && j + 1 < count[t]) {  // S_t = Q_t K^T
-                        const uint32_t n = gone + nth(t, j + 1), st = n % STAGES;
-                        ok = mbar_wait_warp(k_full + st, (n / STAGES) & 1);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t q_addr = smem_u32(q_s + (MODE == TA_PAIR ? t : 0) * kboxes * T::Q_BOX), k_addr = smem_u32(k_s + st * kboxes * T::KV_BOX);
-                        if (elect_one()) {
-                            for (int k = 0; k < c.dim / 16; ++k)
-                                umma_bf16(tmem + t * 128, umma_desc_sw128(q_addr + (k >> 2) * T::Q_BOX + (k & 3) * 32), umma_desc_sw128(k_addr + (k >> 2) * T::KV_BOX + (k & 3) * 32), idesc_s,
-                                          k > 0 ? 1u : 0u);
-                            umma_commit(s_full + t);
-                            if (MODE != TA_PAIR || t == 1 || count[1] == 0) umma_commit(k_empty + st);
-                            if (nth(t, j + 1) + 1 == s.blocks && (MODE != TA_PAIR || t == 1 || count[1] == 0)) umma_commit(&q_empty);  // the segment's last scores
-                        }
-                        __syncwarp();
+                    for (int t = 0; t < T::GROUPS; ++t) {
+                        ok = ok && (j < 0 || j >= count[t] || outputs(t, j));
+                        ok = ok && (j + 1 >= count[t] || scores(t, j + 1));
                     }
                 }
                 if (!ok || __any_sync(0xffffffffu, fail)) { fail = 1; ok = false; }
@@ -385,7 +417,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
     } else {
         const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, copy = row / T::ROWS, in = row % T::ROWS, col0 = copy * T::COLS;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_addr = tmem + t * 128 + lanes;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const float scale2 = a.scale * TA_LOG2E;
         const bool fixes = MODE != TA_PAIR || t == 0;  // of two tiles the first one's products come first
         uint32_t seen = 0, used[2] = {0, 0}, joined = 0;  // blocks of this group, segments of each group, segments in which both had blocks
@@ -405,7 +437,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             for (int n = 0; n < count; ++n) {
                 const int block = s.block0 + nth(t, n), base = block * KEYS;
                 const uint32_t number = gone + nth(t, n), st = number % STAGES;
-                if (!mbar_wait(s_full + t, seen & 1) || fail) { ok = false; break; }
+                const uint32_t buffer = T::SCORES == 2 ? seen & 1 : 0, s_addr = tmem + t * 128 + buffer * 64 + lanes;
+                if (!mbar_wait(&s_full[t][buffer], (T::SCORES == 2 ? seen >> 1 : seen) & 1) || fail) { ok = false; break; }
                 ++seen;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t there = ~0u;
@@ -440,6 +473,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (n == 0) {
                         m = most;
                     } else if (__any_sync(0xffffffffu, most > m + TA_SLACK)) {
+                        if (T::SCORES == 2) {  // the product before this block's may still be adding
+                            if (!__all_sync(0xffffffffu, mbar_wait(pv_done + t, (seen - 2) & 1))) ok = false;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
                         const float next = fmaxf(m, most), fix = next == -INFINITY ? 1.f : ta_exp2(m - next);
                         m = next;
                         l *= fix;
@@ -500,7 +537,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + t);
+                if (lane == 0) mbar_arrive(&p_full[t][buffer]);
+                if (!ok) break;
             }
             // the output of the segment: group 0 of a single tile takes what group 1 has along
             if (MODE == TA_SINGLE && t == 1) {
@@ -776,7 +814,7 @@ static int tree_launch(const TreeAttentionArgs& a, const TreeShape& sh, cudaStre
         if (e != cudaSuccess) return (int)e;
         once.mark(dev);
     }
-    GLMB_LAUNCH((tree_attention_kernel<MODE, COPIES, JOINS>), sh.ctas, TA_THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
+    GLMB_LAUNCH((tree_attention_kernel<MODE, COPIES, JOINS>), sh.ctas, T::THREADS, T::SMEM, stream, map_q, map_k, map_v, a, sh, first_k, first_v, chunk);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || sh.whole) return (int)e;
     const int heads_at_once = min(ceil_div(a.H, 8), ceil_div(148 * 2, a.rows));
