@@ -94,7 +94,7 @@ def append(qkv: torch.Tensor, cache: PagedKV, positions: torch.Tensor | None, se
         if positions is None:
             raise ValueError("a rotation needs positions")
         _check_index("positions", positions, rows, torch.int32, device)
-        if rot.dim() != 3 or rot.shape[2] != 2 or not 0 < 2 * rot.shape[1] <= dim or rot.dtype is not torch.float32 or not rot.is_contiguous() or rot.get_device() != device:
+        if rot.dim() != 3 or not rot.shape[0] or rot.shape[2] != 2 or not 0 < 2 * rot.shape[1] <= dim or rot.dtype is not torch.float32 or not rot.is_contiguous() or rot.get_device() != device:
             raise ValueError("rot is [positions, n, 2] in fp32, contiguous, with 2 n channels at most as many as a head has")
     if status is not None:
         _check_index("status", status, 1, torch.int32, device)
@@ -106,6 +106,8 @@ def append(qkv: torch.Tensor, cache: PagedKV, positions: torch.Tensor | None, se
         return q if want_q else None
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         raise ValueError("rows of qkv are contiguous and 16-byte aligned")
+    if any(t is not None and t.data_ptr() % 16 for t in (rot, q_norm, k_norm)):
+        raise ValueError("rot and the weights of the norms begin at a 16-byte boundary")
     with native.on_device(qkv):
         q = qkv.new_empty((rows, heads, dim)) if want_q else None
         native.paged_append(qkv, args, positions, seqs, slots, q, heads, rot, pairs, q_norm, k_norm, eps, status=status)

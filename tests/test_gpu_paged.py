@@ -65,6 +65,38 @@ def test_append(native_lib, rows, H, G, dim, vdim, page, rot, norm, pairs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("rows, H, G, dim, rot", [(40, 9, 2, 64, 24), (3, 70, 8, 128, 40), (11, 5, 5, 48, 20), (2, 33, 1, 256, 248), (6, 4, 2, 32, 2)])
+def test_append_turns_part_of_a_head(native_lib, rows, H, G, dim, rot, pairs):
+    for norm in (True, False):
+        assert_append(append_case(rows, H, G, dim, dim, 8, rot=rot, norm=norm), pairs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("rot, at", [(16, 16), (16, 23), (12, 12), (12, 14), (10, 10), (0, 9)])
+def test_append_keeps_an_infinity_that_does_not_turn_to_itself(native_lib, rot, at, pairs):
+    c = append_case(5, 2, 1, 32, 32, 8, rot=rot, norm=False)
+    q, d = run_append(cuda(c), pairs=pairs), None
+    c["qkv"][1, at] = math.inf
+    d = cuda(c)
+    with_inf = run_append(d, pairs=pairs)
+    assert float(with_inf[1, 0, at]) == math.inf
+    with_inf[1, 0, at] = q[1, 0, at]
+    assert torch.equal(with_inf, q)
+
+
+@pytest.mark.gpu
+def test_append_refuses_what_its_loads_cannot_take(native_lib):
+    d = cuda(append_case(4, 2, 1, 32, 32, 8, rot=16))
+    odd = torch.ones(40, dtype=torch.bfloat16, device="cuda")[1:33]
+    far = torch.zeros(4 * 8 * 2 + 2, device="cuda")[2:].view(4, 8, 2)
+    for more in (dict(q_norm=odd), dict(k_norm=odd), dict(rot=far), dict(rot=d["rot"][:0])):
+        with pytest.raises(ValueError):
+            run_append(d, **more)
+
+
+@pytest.mark.gpu
 def test_append_strides_layouts_and_rows_without_a_slot(native_lib):
     c = append_case(9, 8, 2, 64, 64, 16, rot=32)
     c["slots"][4] = -1

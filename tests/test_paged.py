@@ -77,7 +77,7 @@ def test_refusals():
     rot = torch.zeros(9, 8, 2)
     app = lambda *a, **more: lambda: paged.append(*(a or (qkv, c, one, one, one)), **({"heads": 4} | more))  # noqa: E731
     bad += [app(status=torch.zeros(1)), app(heads=3), app(heads=0), app(qkv.float(), c, one, one, one), app(qkv, c, one, one[:1], one), app(qkv, c, one, one, one.long()), app(qkv, c, None, one, one, rot=rot),
-            app(rot=rot.double()), app(rot=torch.zeros(9, 9, 2)), app(rot=torch.zeros(9, 0, 2)), app(q_norm=torch.ones(16)), app(k_norm=torch.ones(8).bfloat16())]
+            app(rot=rot.double()), app(rot=torch.zeros(9, 9, 2)), app(rot=torch.zeros(9, 0, 2)), app(rot=torch.zeros(0, 8, 2)), app(q_norm=torch.ones(16)), app(k_norm=torch.ones(8).bfloat16())]
     for call in bad:
         with pytest.raises(ValueError):
             call()
