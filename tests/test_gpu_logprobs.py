@@ -209,6 +209,33 @@ def test_head_in_fp32(native_lib, rows):
     check_head(logprobs.head_logprobs(hidden.cuda(), head.cuda(), tokens.cuda()), hidden, head, tokens)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 20, 200])
+def test_head_table_of_more_than_32_bits(native_lib, rows):
+    """2^31 elements and more; but for its last 64 tokens the table is zeros, so those tokens' logits are."""
+    width, few = 8192, 64
+    vocab = (1 << 31) // width + 200
+    g = torch.Generator().manual_seed(rows)
+    last = (torch.randn(few, width, generator=g) * 4 * width**-0.5).bfloat16()
+    head = torch.zeros(vocab, width, dtype=torch.bfloat16, device="cuda")
+    head[-few:] = last.cuda()
+    k = torch.randint(0, few, (rows,), generator=g)
+    hidden = (torch.randn(rows, width, generator=g) + 2.0 * last[k].float()).bfloat16()
+    got = logprobs.head_logprobs(hidden.cuda(), head, (vocab - few + k).cuda())
+    x = hidden.double() @ last.double().T
+    lse = torch.logaddexp(torch.logsumexp(x, 1), torch.tensor(math.log(vocab - few), dtype=torch.float64))
+    # the zeros: a thread of the widest run adds 1,024 terms of them one after another, so (1,024 + 16) 2^-24 takes the place of 144 2^-24 in the bound
+    bound = (1040 + 4) * 2.0**-24 + 32 * 2.0**-23 + 2 * (width + 16) * 2.0**-23 * (hidden.double().abs() @ last.double().abs().T).amax(1) + 2.0**-21 * lse.abs()
+    assert bool(((got.logprob.cpu().double() - (x[torch.arange(rows), k] - lse)).abs() <= bound).all())
+    assert bool(((got.best.cpu().double() - (x.amax(1) - lse)).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_many_rows(native_lib):
+    x, tokens = rows_of(70001, 37, torch.bfloat16)
+    check(logprobs.token_logprobs(x.cuda(), tokens.cuda(), top=2), x, tokens, 2)
+
+
 # ------------------------------------------------------------------------------------------------ streams and graphs
 @pytest.mark.gpu
 def test_on_a_stream_of_its_own_and_in_two_graphs(native_lib):

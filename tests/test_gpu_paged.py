@@ -322,6 +322,13 @@ def test_offsets_beyond_32_bits(native_lib):
     assert torch.equal(k[table[0, 1].item(), 101 - 64].flatten(), qkv[0, 8 * dim : 16 * dim]) and torch.equal(v[table[0, 1].item(), 101 - 64].flatten(), qkv[0, 16 * dim :])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs, length, tree", [(700, 9, 1), (300, 700, 2), (1500, 0, 3)])
+def test_many_sequences(native_lib, seqs, length, tree):
+    case = tree_case([(length * (b % 7)) // 6 for b in range(seqs)], [1 + b % tree for b in range(seqs)], H=4, G=2, dim=32, vdim=32, page=8)
+    assert_tree(paged.tree_attention(**to_cuda(case)), case)
+
+
 # ------------------------------------------------------------------------------------------------ the operators together
 def _step(p, cache, starts, lengths, masks, positions, seqs, slots, tokens, status):
     """One step over drafted tokens: projection -> append -> attention -> projection -> log probabilities."""
