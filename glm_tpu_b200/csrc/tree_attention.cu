@@ -22,7 +22,7 @@
 // The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
 // (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-8 each beside that of the result.  What
 // bounds them is one warp that issues for both: a block of 128 keys of two tiles takes 2.7 thousand cycles of softmax (2.0 of them exponentials) and 1.9 until
-// the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 4 heads at 131,000 slots: 296 us, 303 before
+// the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 8 heads at 131,000 slots: 296 us, 303 before
 // the softmax threads got the registers that their scores need (167 -> 157 for 4 x 64 drafts at 30,000).  Measured beside those 303: two buffers of scores, blocks
 // of 64 keys 424 us, with two issuing warps 303; blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
 // A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; memory is its bound, so its weights
