@@ -119,7 +119,7 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
     typedef HeadCta<PAIR> C;
     GLMB_PDL_PROLOGUE();
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[HL_STAGES], empty[HL_STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full[HL_STAGES], empty[HL_STAGES], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t fail;
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -131,6 +131,7 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; ++s) mbar_init(full + s, 1), mbar_init(empty + s, 1);
         for (int a = 0; a < 2; ++a) mbar_init(acc_full + a, 1), mbar_init(acc_empty + a, PAIR ? 16 : 8);
+        mbar_init(&drained, 1);
         fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,7 +151,8 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0) {
-        HeadRing g;
+        HeadRing g, last;  // last: the place of the last stage but plan.stages
+        int issued = 0;
         bool ok = true;
         HeadTile t;
         for (int n = 0; ok && hl_tile(plan, p.vocab, worker, n, t); ++n) {
@@ -169,8 +171,11 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
                         for (int r = 0; r < mine; r += HL_BOX) C::load(dst + a_bytes + r * 128, &map_rest, full + s, kb * 64, b_row + r);
                 }
                 __syncwarp();
+                if (++issued > plan.stages) last.next(plan.stages);
             }
         }
+        // nobody leaves while copies are under way, not after a timeout either (of a pair the first CTA knows)
+        for (int i = min(issued, plan.stages); rank == 0 && i > 0; --i, last.next(plan.stages)) mbar_wait_warp(full + last.at, last.lap & 1);
     } else if (warp == 1) {
         HeadRing g;
         uint32_t used = 0;  // accumulators so far
@@ -200,6 +205,9 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
                 __syncwarp();
             }
         }
+        if (rank == 0 && elect_one()) C::commit(&drained);  // nor while products are
+        __syncwarp();
+        mbar_wait_warp(&drained, 0);
     } else {
         const int quarter = warp & 3, half = warp >= 6;
         const uint32_t at = tmem + half * 128 + ((uint32_t)(quarter * 32) << 16);

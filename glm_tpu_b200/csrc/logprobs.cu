@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(LP_THREADS + 32, 4) token_logprobs_kernel(Toke
     float token_logit = 0.f;
     if (warp == LP_WARPS) {
         if (lane == 0) {
-            for (int i = 0; i < stages; ++i) {
+            int i = 0;
+            for (; i < stages; ++i) {
                 const int s = i % LP_STAGES, lap = i / LP_STAGES, at = begin + i * LP_STAGE;
                 if (lap > 0 && !mbar_wait(empty + s, (lap - 1) & 1)) break;  // the others' waits run out too, and say so
                 const uint32_t bytes = (uint32_t)min(LP_STAGE, end - at) * 16;
@@ -210,6 +211,7 @@ __global__ void __launch_bounds__(LP_THREADS + 32, 4) token_logprobs_kernel(Toke
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                              ::"r"(smem_u32(ring + s * LP_STAGE)), "l"(v + at), "r"(bytes), "r"(smem_u32(full + s)) : "memory");
             }
+            for (int k = max(0, i - LP_STAGES); k < i; ++k) mbar_wait(full + k % LP_STAGES, (k / LP_STAGES) & 1);  // nobody leaves while copies are under way
         }
         __syncwarp();
     } else {

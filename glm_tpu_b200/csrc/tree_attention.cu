@@ -203,7 +203,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     constexpr int KEYS = T::KEYS, STAGES = T::STAGES, WORDS = KEYS / 32;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-    __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], ml_full;  // of a group (and of its buffer of scores)
+    __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], ml_full, drained;  // of a group (and of its buffer of scores)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t fail;
     __shared__ uint32_t page_bits[TA_NOTES][WORDS];  // keys of a block whose page exists
@@ -219,7 +219,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     float* join_s = reinterpret_cast<float*>(v_s + STAGES * T::BOXES * T::KV_BOX);
 
     if (threadIdx.x == 0) {
-        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&ml_full, 4);
+        mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&ml_full, 4), mbar_init(&drained, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(o_full + i, 1), mbar_init(o_free + i, 4), mbar_init(pv_done + i, 1);
             for (int e = 0; e < 2; ++e) mbar_init(&s_full[i][e], 1), mbar_init(&p_full[i][e], 4);
@@ -299,11 +299,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const bool slots_first = keys ? slots_first_k : slots_first_v;
         unsigned char* ring = keys ? k_s : v_s;
         uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+        uint32_t issued = 0;  // blocks
+        int queries = 0;
         bool ok = true;
         for (; ok && walk.next(a, sh, s); gone += s.blocks, ++segment) {
             if (keys) {
                 if (segment > 0 && !mbar_wait_warp(&q_empty, (segment - 1) & 1)) { fail = 1; break; }
                 const int tiles = MODE == TA_PAIR ? min(2, sh.tiles(s.seq.rows) - s.unit * 2) : 1;
+                ++queries;
                 if (lane == 0) broken[segment & 3] = 0;
                 __syncwarp();
                 if (elect_one()) {
@@ -346,8 +349,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         ta_tma_4d(ring + (st * boxes + x) * T::KV_BOX + lane * chunk * 128, map, full + st, x * 64, slots_first ? in_page : s.g, slots_first ? s.g : in_page, page);
                 __syncwarp();
                 page = next_page;
+                ++issued;
             }
         }
+        // nobody leaves while copies are under way, not after a timeout either
+        for (uint32_t n = issued > STAGES ? issued - STAGES : 0; n < issued; ++n) mbar_wait_warp(full + n % STAGES, (n / STAGES) & 1);
+        if (queries) mbar_wait_warp(&q_full, (queries - 1) & 1);
     } else if (warp == 8) {
         const uint32_t idesc_s = umma_idesc_bf16(128, KEYS), idesc_o = umma_idesc_bf16(128, c.vdim) | (1u << 16);  // bit 16: B is MN-major
         uint32_t made[2] = {0, 0}, done[2] = {0, 0}, uses[2] = {0, 0};  // blocks of scores, of outputs, and segments of a group so far
@@ -415,6 +422,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (!ok || __any_sync(0xffffffffu, fail)) { fail = 1; ok = false; }
             }
         }
+        if (elect_one()) umma_commit(&drained);  // nor while products are
+        __syncwarp();
+        mbar_wait_warp(&drained, 0);
     } else {
         const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, copy = row / T::ROWS, in = row % T::ROWS, col0 = copy * T::COLS;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
