@@ -46,16 +46,17 @@ def ancestor_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
     return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64), torch.tensor(depths, dtype=torch.int32)
 
 
-def _checked(cache: PagedKV, device: int) -> native.PagedArgs:
-    """The cache as the kernels take it; ``device``: where the rows lie (-1: CPU)."""
+def _checked(cache: PagedKV, device: int) -> tuple[int, ...]:
+    """The cache as the kernels take it (the fields of ``native.PagedArgs``; the last seven: sequences, their pages, pages, slots of a page, heads, dim, vdim).
+    ``device``: where the rows lie (-1: CPU)."""
     k, v, table = cache.k, cache.v, cache.table
     if k.dim() != 4 or v.dim() != 4 or table.dim() != 2:
         raise ValueError("pools have four axes, the table two")
     pages, page, G, dim = k.shape
-    vdim, (seqs, per_seq) = v.shape[3], table.shape
+    (*v_front, vdim), (seqs, per_seq) = v.shape, table.shape
     k_page, k_slot, k_head, k_last = k.stride()
     v_page, v_slot, v_head, v_last = v.stride()
-    if v.shape[:3] != k.shape[:3] or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or not pages or not page or page % 8 or not G:
+    if v_front != [pages, page, G] or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or not pages or not page or page % 8 or not G:
         raise ValueError("pools are [pages, page, kv_heads, dim] and [pages, page, kv_heads, vdim] in bf16, with a multiple of 8 slots a page")
     if table.dtype is not torch.int32 or (per_seq > 1 and table.stride(1) != 1) or per_seq * page > MAX_SLOTS:
         raise ValueError("the table is [sequences, pages of a sequence] in int32, of up to 2^30 slots a sequence")
@@ -66,7 +67,7 @@ def _checked(cache: PagedKV, device: int) -> native.PagedArgs:
     k_at, v_at = k.data_ptr(), v.data_ptr()
     if device >= 0 and (k_last != 1 or v_last != 1 or (k_page | k_slot | k_head | v_page | v_slot | v_head) % 8 or (k_at | v_at) % 16):
         raise ValueError("the channels of a head are contiguous and every head of the pools 16-byte aligned")
-    return native.PagedArgs(k_at, k_page, k_slot, k_head, v_at, v_page, v_slot, v_head, table.data_ptr(), table.stride(0), seqs, per_seq, pages, page, G, dim, vdim)
+    return k_at, k_page, k_slot, k_head, v_at, v_page, v_slot, v_head, table.data_ptr(), table.stride(0), seqs, per_seq, pages, page, G, dim, vdim
 
 
 def _check_index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: int) -> None:
@@ -84,8 +85,8 @@ def append(qkv: torch.Tensor, cache: PagedKV, positions: torch.Tensor | None, se
     slots.  ``want_q=False``: keys and values only (returns ``None``)."""
     device = qkv.get_device()
     args = _checked(cache, device)
-    dim = args.dim
-    if qkv.dim() != 2 or qkv.dtype is not torch.bfloat16 or heads < 1 or qkv.shape[1] != heads * dim + args.G * (dim + args.vdim):
+    G, dim, vdim = args[-3:]
+    if qkv.dim() != 2 or qkv.dtype is not torch.bfloat16 or heads < 1 or qkv.shape[1] != heads * dim + G * (dim + vdim):
         raise ValueError("qkv is [rows, heads * dim + kv_heads * (dim + vdim)] in bf16")
     rows = qkv.shape[0]
     _check_index("seqs", seqs, rows, torch.int32, device)
@@ -124,8 +125,8 @@ def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, length
     that sees nothing, without a sink, is zeros.  Rows that belong to no sequence stay as they are in ``out``, or are zeros where it is made here."""
     device = q.get_device()
     args = _checked(cache, device)
-    seqs, vdim = args.seqs, args.vdim
-    if q.dim() != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != args.dim or not q.shape[1] or q.shape[1] % args.G:
+    seqs, _, _, _, G, dim, vdim = args[-7:]
+    if q.dim() != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != dim or not q.shape[1] or q.shape[1] % G:
         raise ValueError("q is [rows, heads, dim] in bf16, with a multiple of the cache's heads")
     rows, heads, _ = q.shape
     if seqs > 65535:

@@ -10,6 +10,7 @@ fails on a GPU machine the call raises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import torch
@@ -190,6 +191,23 @@ class TreeAttentionArgs(C.Structure):
         ("status", C.c_void_p),
     ]
 
+
+def _packer(kind):
+    """``pack(*values)``: a structure as bytes, the fields of nested ones in line, null pointers 0.  Building the structure itself takes three times as long (2.0 us
+    for the arguments of an append, 0.7 so), which shows where a launch waits for the host."""
+    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f"}
+
+    def fields(of):  # 0P: nested structures begin and end where a pointer may lie
+        return "".join(f"0P{fields(t)}0P" if issubclass(t, C.Structure) else codes[t] for _, t in of._fields_)
+
+    packed = struct.Struct(f"@{fields(kind)}0P")
+    if packed.size != C.sizeof(kind):
+        raise TypeError(f"{kind.__name__} has fields that are not packed as the compiler does")
+    return packed.pack
+
+
+_pack_token_logprobs, _pack_head_logprobs = _packer(TokenLogprobsArgs), _packer(HeadLogprobsArgs)
+_pack_append, _pack_tree = _packer(PagedAppendArgs), _packer(TreeAttentionArgs)
 
 # argument structures and the entry point that gives their size in the library
 _STRUCTS = (("glmb_qkv_conv_args_sizeof", QkvConvArgs), ("glmb_chunk_attn_args_sizeof", ChunkAttnArgs), ("glmb_latent_args_sizeof", LatentArgs),
@@ -905,18 +923,23 @@ def step_finalize(cand, n_sets, rows, row_active, tokens, positions, out_tokens,
 
 
 # ----------------------------------------------------------------------------- log probabilities of given tokens
-def _scores(tokens, sums, status) -> TokenScores:
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _scores(tokens, sums, status):
+    """The fields of ``TokenScores``."""
     out, item = sums.data_ptr(), sums.stride(0) * 4
-    return TokenScores(tokens.data_ptr(), out, out + item, out + 2 * item, tokens.dtype == torch.int64, None if status is None else status.data_ptr())
+    return tokens.data_ptr(), out, out + item, out + 2 * item, tokens.dtype is torch.int64, _ptr(status)
 
 
 def token_logprobs(logits, tokens, sums, top_ids=None, top_logprobs=None, *, status=None):
     """``sums`` fp32 ``[3, rows]``: log probability of ``tokens`` (int32 or int64), entropy, log probability of the most likely token; with ``top_ids``
     int32 and ``top_logprobs`` fp32 ``[rows, top]`` the most likely tokens, ties to the lowest id.  bf16 or fp32 logits, one pass."""
     rows, vocab = logits.shape
-    a = TokenLogprobsArgs(logits.data_ptr(), logits.stride(0), _scores(tokens, sums, status), None if top_ids is None else top_ids.data_ptr(),
-                          None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab, 0 if top_ids is None else top_ids.shape[1], logits.dtype == torch.float32)
-    _check(lib().glmb_token_logprobs(C.byref(a), _stream()), "token_logprobs")
+    a = _pack_token_logprobs(logits.data_ptr(), logits.stride(0), *_scores(tokens, sums, status), _ptr(top_ids), _ptr(top_logprobs), rows, vocab,
+                             0 if top_ids is None else top_ids.shape[1], logits.dtype is torch.float32)
+    _check(lib().glmb_token_logprobs(a, _stream()), "token_logprobs")
 
 
 HEAD_SLAB = 1 << 26  # fp32: logits of a slab of rows
@@ -931,9 +954,9 @@ def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
         parts = _lib.glmb_head_logprobs_parts(rows, vocab)  # not a launch: past the wrapper that times launches
         room = torch.empty((4 * parts + 1) * rows, dtype=torch.float32, device=hidden.device)
         part = room.data_ptr()
-        a = HeadLogprobsArgs(hidden.data_ptr(), hidden.stride(0), head.data_ptr(), head.stride(0), _scores(tokens, sums, status), part, part + 16 * parts * rows, parts,
-                             rows, vocab, width)
-        _check(lib().glmb_head_logprobs(C.byref(a), _stream()), "head_logprobs")
+        a = _pack_head_logprobs(hidden.data_ptr(), hidden.stride(0), head.data_ptr(), head.stride(0), *_scores(tokens, sums, status), part, part + 16 * parts * rows, parts,
+                                rows, vocab, width)
+        _check(lib().glmb_head_logprobs(a, _stream()), "head_logprobs")
         return
     step = rows if hidden.dtype == torch.bfloat16 else max(1, min(rows, HEAD_SLAB // vocab))
     logits = torch.empty((step, -(-vocab // 8) * 8), dtype=torch.float32, device=hidden.device)
@@ -947,34 +970,32 @@ def head_logprobs(hidden, head, vocab, tokens, sums, *, status=None):
 
 
 # ----------------------------------------------------------------------------- drafted tokens over a paged cache
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def paged_append(qkv, cache: PagedArgs, positions, seqs, slots, q, heads, rot=None, pairs=False, q_norm=None, k_norm=None, eps=1e-6, *, status=None):
-    """Norm and rotation of the heads of a fused projection; keys and values into the pages of their slots (``layers.attention.paged.append``)."""
+def paged_append(qkv, cache, positions, seqs, slots, q, heads, rot=None, pairs=False, q_norm=None, k_norm=None, eps=1e-6, *, status=None):
+    """Norm and rotation of the heads of a fused projection; keys and values into the pages of their slots (``layers.attention.paged.append``).  ``cache``: the
+    fields of ``PagedArgs``."""
     half, angles = (0, 0) if rot is None else (rot.shape[1], rot.shape[0])
-    a = PagedAppendArgs(cache, qkv.data_ptr(), qkv.stride(0), _ptr(q_norm), _ptr(k_norm), _ptr(rot), 2 * half, angles, pairs, _ptr(positions), seqs.data_ptr(), slots.data_ptr(),
-                        _ptr(q), heads * cache.dim, qkv.shape[0], heads, eps, _ptr(status))
-    _check(lib().glmb_paged_append(C.byref(a), _stream()), "paged_append")
+    a = _pack_append(*cache, qkv.data_ptr(), qkv.stride(0), _ptr(q_norm), _ptr(k_norm), _ptr(rot), 2 * half, angles, pairs, _ptr(positions), seqs.data_ptr(), slots.data_ptr(),
+                     _ptr(q), heads * cache[-2], qkv.shape[0], heads, eps, _ptr(status))
+    _check(lib().glmb_paged_append(a, _stream()), "paged_append")
 
 
-def tree_attention(q, cache: PagedArgs, starts, lengths, masks, scale, max_rows, sink, out, *, clear_rest=False, status=None):
-    """Attention of drafted rows over a paged cache and their ancestors (``layers.attention.paged.tree_attention``)."""
+def tree_attention(q, cache, starts, lengths, masks, scale, max_rows, sink, out, *, clear_rest=False, status=None):
+    """Attention of drafted rows over a paged cache and their ancestors (``layers.attention.paged.tree_attention``).  ``cache``: the fields of ``PagedArgs``."""
     rows, H, _ = q.shape
     q_row, q_head, _ = q.stride()
     out_row, out_head, _ = out.stride()
-    a = TreeAttentionArgs(cache, q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, starts.data_ptr(), lengths.data_ptr(), masks.data_ptr(), _ptr(sink), None, None, 0,
-                          rows, H, max_rows, scale, clear_rest, _ptr(status))
-    launch = lib().glmb_tree_attention
-    parts = _lib.glmb_tree_attention_parts(C.byref(a))  # not a launch: past the wrapper that times launches
+    front = (*cache, q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, starts.data_ptr(), lengths.data_ptr(), masks.data_ptr(), _ptr(sink))
+    back = rows, H, max_rows, scale, clear_rest, _ptr(status)
+    a = _pack_tree(*front, 0, 0, 0, *back)
+    launch, vdim = lib().glmb_tree_attention, cache[-1]
+    parts = _lib.glmb_tree_attention_parts(a)  # not a launch: past the wrapper that times launches
     if parts < 0:
         raise ValueError("tree_attention: sizes that the kernels do not take")
     if parts:  # sums of keys that several CTAs share
-        room = torch.empty(parts * (cache.vdim + 2), dtype=torch.float32, device=q.device)
-        a.part_o = room.data_ptr()
-        a.part_ml, a.parts = a.part_o + 4 * parts * cache.vdim, parts
-    _check(launch(C.byref(a), _stream()), "tree_attention")
+        room = torch.empty(parts * (vdim + 2), dtype=torch.float32, device=q.device)
+        at = room.data_ptr()
+        a = _pack_tree(*front, at, at + 4 * parts * vdim, parts, *back)
+    _check(launch(a, _stream()), "tree_attention")
 
 
 def fp8_to_bf16(bits, scale, out, block=(128, 128), status=None):
