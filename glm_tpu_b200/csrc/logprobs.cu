@@ -23,6 +23,7 @@ namespace cg = cooperative_groups;
 #define LP_STAGE 1024  // vectors (16 KB) of a stage of the ring
 #define LP_STAGES 3
 #define LP_RING (LP_STAGES * LP_STAGE * 16)
+#define LP_SM 233472   // bytes of shared memory of an SM
 #define LP_PARTS 8     // CTAs of a row, at most
 
 struct TokenLogprobsArgs {
@@ -352,14 +353,18 @@ GLMB_API int glmb_token_logprobs(const TokenLogprobsArgs* args, cudaStream_t str
     if (a.rows < 0 || a.vocab < 1 || a.vocab > 0x7ffffff0 || a.top < 0 || a.top > LP_TOP || a.top > a.vocab || a.stride < 0 || a.rows > 0x7fffffff / LP_PARTS) return 1;
     if (a.rows == 0) return 0;
     // CTAs of a row: as many as run at once (three to four an SM), with 2,048 logits or more each.  Every CTA has its start, its bound and its merge to pay for:
-    // 333 rows of 65,521 in fp32, five alternatives, 1 - 8 CTAs a row: 33, 35, 40, 51 us; 108 of 82,183: 25, 25, 20 (432 CTAs), 26; 10 of 45,744: 15.6, 11.4, 9.1, 7.5;
-    // one of 154,880 in bf16 with twenty: 33, 23, 16, 12.
+    // 333 rows of 65,521 in fp32, five alternatives, 1, 2, 4 and 8 CTAs a row: 28.6, 34.5, 40, 50 us; 108 of 82,183: 23, 20, 20, 26; 40 of 154,880 in bf16: 32, 22, 17,
+    // 15.6; one with twenty: 33, 23, 15.7, 12.3.
     int parts = 1;
     while (parts < LP_PARTS && (int64_t)a.rows * parts * 2 <= 148 * 3 && a.vocab / (2 * parts) >= 2048) parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * parts));
     cfg.blockDim = dim3(LP_THREADS + 32);
-    cfg.dynamicSmemBytes = LP_RING;
+    // Evenly over the SMs: left to themselves four CTAs go to one while another has two, so each asks for as much shared memory as keeps a further one away (333
+    // rows 33.1 -> 28.6 us, 200 rows 23.0 -> 20.4, 30 rows in eights 13.8 -> 11.7).  Clusters lie in one of eight groups of SMs, each of which may have parts - 1
+    // places over: without room for them 16 rows in eights go in two rounds (11.1 -> 17.6).
+    const int per_sm = ceil_div(a.rows * parts + (parts > 2 ? 8 * (parts - 1) : 0), 148);
+    cfg.dynamicSmemBytes = per_sm < 4 ? LP_SM / (per_sm + 1) : LP_RING;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -375,7 +380,7 @@ GLMB_API int glmb_token_logprobs(const TokenLogprobsArgs* args, cudaStream_t str
     if (dev != DeviceOnce::SET) {
         for (const void* k : {(const void*)token_logprobs_kernel<float, true>, (const void*)token_logprobs_kernel<float, false>, (const void*)token_logprobs_kernel<bf16, true>,
                               (const void*)token_logprobs_kernel<bf16, false>}) {
-            e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_RING);
+            e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SM / 2);
             if (e != cudaSuccess) return (int)e;
         }
         once.mark(dev);
