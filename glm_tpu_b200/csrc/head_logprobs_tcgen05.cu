@@ -6,8 +6,8 @@
 // of the table in L2; where the workers divide among the row blocks with little left over, each keeps its row block and its sums in registers until
 // the end, else it leaves the sums of every tile.  A second launch joins them, a warp a row.
 //
-// Bound: up to some 150 rows the table's bytes (16 rows of 4,096 against 131,072 tokens 168 us, 6.4 TB/s), above that the tensor core (2,048 rows 1,570 - 1,660 us, 1,325 - 1,400
-// TFLOP/s by the power the chip may draw), with narrow hidden states the sums (1,024 rows of 512: 124 - 174 us).
+// Bound: up to some 150 rows the table's bytes (16 rows of 4,096 against 131,072 tokens 168 us, 6.4 TB/s), above that the tensor core (2,048 rows 1,570 -
+// 1,660 us, 1,325 - 1,400 TFLOP/s by the power the chip may draw), with narrow hidden states the sums (1,024 rows of 512: 124 - 174 us).
 //
 // The tensor core does not round its running sum to nearest: over K = 4,096 that is a bias of 3.7e-6 of a logit, eight times what fp32 loses otherwise.  So
 // a sum stays there for 512 products only; the epilogue's threads keep their 128 logits in registers and add (at K = 512 the bias is 3.5e-7).  TMEM holds two

@@ -19,15 +19,15 @@
 // A tile of up to 64 or 32 pairs is there two or four times among the 128 rows: each copy weighs its own half or quarter of every block (its weights of the rest
 // are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs, or in shared memory.
 //
-// The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a unit
-// (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-8 each beside that of the result.  What
-// bounds them is one warp that issues for both: a block of 128 keys of two tiles takes 2.7 thousand cycles of softmax (2.0 of them exponentials) and 1.9 until
-// the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 8 heads at 131,000 slots: 296 us, 303 before
-// the softmax threads got the registers that their scores need (167 -> 157 for 4 x 64 drafts at 30,000).  Measured beside those 303: two buffers of scores, blocks
-// of 64 keys 424 us, with two issuing warps 303; blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
-// A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; memory is its bound, so its weights
-// keep a second piece, the remainder of the first.  Heads wider than 128 (WIDE): blocks of 64 keys, one group, and two buffers of scores, so that the next ones are there
-// when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer 320).
+// The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a
+// unit (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-8 each beside that of the
+// result.  What bounds them is one warp that issues for both: a block of 128 keys of two tiles takes 2.7 thousand cycles of softmax (2.0 of them exponentials)
+// and 1.9 until the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 8 heads at 131,000 slots: 296 us, 303
+// before the softmax threads got the registers that their scores need (167 -> 157 for 4 x 64 drafts at 30,000).  Measured beside those 303: two buffers of
+// scores, blocks of 64 keys 424 us, with two issuing warps 303; blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
+// A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; its weights keep a second piece, the
+// remainder of the first (one piece: 108 -> 101 us for 4 x 16 drafts at 30,000).  Heads wider than 128 (WIDE): blocks of 64 keys, one group, and two buffers of
+// scores, so that the next ones are there when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer 320).
 //
 //   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
 //   warp 8           issues every tcgen05.mma, owns the TMEM allocation
