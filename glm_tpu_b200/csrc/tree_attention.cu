@@ -53,6 +53,8 @@
 #define TA_SLACK 8.0f     // log2 of how far the weights may exceed one before the maximum is followed
 #define TA_JOIN 68        // floats of a row of joined sums: 64 columns, padded
 #define TA_WHOLE_BLOCKS 4 // caches of so few blocks a sequence: units are not split
+#define TA_LONG_RUN 8     // blocks a CTA from which on the start of a unit counts
+#define TA_START 4        // as so many
 #define TA_NOTES 8        // blocks whose pages are remembered: the producer is at most five ahead of the softmax
 
 enum { TA_PAIR = 0, TA_SINGLE = 1, TA_WIDE = 2 };
@@ -78,10 +80,13 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttentionArgs& a, int b, b
 struct TreeShape {
     int per, heads, head_blocks, tile_rows, in_unit, copies, keys, ctas, units_max;  // units_max: of a key head of the largest sequence
     int whole;  // runs are whole units, as many for every CTA: nothing is left to join
+    int start;  // blocks that the start of a unit counts for: a CTA's turn from one unit to the next
+    // What a unit counts for in the runs: places, of which the first `start` hold no block.
+    __device__ __forceinline__ int places(const TreeSeq& s) const { return whole ? 1 : s.blocks(keys) + start; }
     // The place of a tile's sums of a segment; a row's lie behind it.
     __device__ __forceinline__ int64_t part(int64_t segment, int tile_of_unit, int copy) const { return ((segment * in_unit + tile_of_unit) * copies + copy) * (heads * tile_rows); }
     // What a sequence's units count for in the runs.
-    __device__ __forceinline__ int64_t share_of(const TreeSeq& s, int G) const { return s.rows ? (int64_t)(whole ? 1 : s.blocks(keys)) * units(s.rows) * G : 0; }
+    __device__ __forceinline__ int64_t share_of(const TreeSeq& s, int G) const { return s.rows ? (int64_t)places(s) * units(s.rows) * G : 0; }
     __device__ __forceinline__ int tiles(int rows) const { return (rows + tile_rows - 1) / tile_rows * head_blocks; }
     __device__ __forceinline__ int units(int rows) const { return (tiles(rows) + in_unit - 1) / in_unit; }
 };
@@ -121,8 +126,8 @@ struct TreeSegment {
 };
 // Walks a run.
 struct TreeWalk {
-    int64_t left;
-    int b, at;  // the sequence, and how many of its (key head, unit) pairs are done
+    int64_t left;  // places
+    int b, at;     // the sequence, and how many of its (key head, unit) pairs are done
     int block0;
     __device__ __forceinline__ bool next(const TreeAttentionArgs& a, const TreeShape& sh, TreeSegment& s) {
         while (left > 0 && b < a.cache.seqs) {
@@ -135,7 +140,7 @@ struct TreeWalk {
             }
             s.b = b, s.g = at / units, s.unit = at % units, s.block0 = block0;
             s.blocks = sh.whole ? s.of : (int)min((int64_t)(s.of - block0), left);
-            left -= sh.whole ? 1 : s.blocks;
+            left -= (sh.whole ? 1 : s.blocks) + sh.start;  // and the places at the start of the next unit
             ++at, block0 = 0;
             return true;
         }
@@ -273,8 +278,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     TreeWalk walk{run_s[0], 0, 0, 0};
     if (walk.left > 0) {
         walk.b = (int)run_s[1];
-        const int of = sh.whole ? 1 : tree_seq(a, walk.b, false).blocks(KEYS);
-        walk.at = (int)(run_s[2] / of), walk.block0 = (int)(run_s[2] % of);
+        const int places = sh.places(tree_seq(a, walk.b, false));
+        const int place = (int)(run_s[2] % places) - sh.start;
+        walk.at = (int)(run_s[2] / places), walk.block0 = max(place, 0), walk.left += min(place, 0);
     }
     // blocks of a segment that group t takes, and the n-th of them (counted from the segment's first)
     auto group_blocks = [&](const TreeSegment& s, int t) {
@@ -716,13 +722,13 @@ __global__ void __launch_bounds__(256, 2) tree_merge_kernel(const __grid_constan
         return;
     }
     const int64_t share = (of.total + sh.ctas - 1) / sh.ctas;
-    const int j = of.j, blocks = of.seq.blocks(sh.keys), units = sh.units(of.seq.rows), row_block = j / sh.tile_rows * sh.head_blocks;
+    const int j = of.j, places = sh.places(of.seq), units = sh.units(of.seq.rows), row_block = j / sh.tile_rows * sh.head_blocks;
     const int rows_of = sh.heads * sh.tile_rows, segment = sh.in_unit * sh.copies * rows_of, shift = sh.copies == 4 ? 2 : sh.copies - 1;
     auto offset = [&](int k) { return (k >> shift) * segment + (k & (sh.copies - 1)) * rows_of; };  // places of the k-th sum behind the first
     for (int h = h0; h < a.H; h += step) {
         const int g = h / sh.per, hh = h % sh.per, tile = row_block + hh / sh.heads, unit = tile / sh.in_unit;
-        const int64_t from = of.upto - (int64_t)blocks * units * c.G + ((int64_t)g * units + unit) * blocks;
-        const int first = (int)(from / share), last = (int)((from + blocks - 1) / share), parts = (last - first + 1) * sh.copies;  // CTAs with keys of the unit
+        const int64_t from = of.upto - (int64_t)places * units * c.G + ((int64_t)g * units + unit) * places;
+        const int first = (int)((from + sh.start) / share), last = (int)((from + places - 1) / share), parts = (last - first + 1) * sh.copies;  // CTAs with keys of the unit
         if (parts == 1) continue;  // written already
         const int64_t place = sh.part(((int64_t)of.b * c.G + g) * sh.units_max + unit + first, tile % sh.in_unit, 0) + j % sh.tile_rows * sh.heads + hh % sh.heads;
         const float* part_ml = a.part_ml + place * 2;
@@ -775,6 +781,9 @@ static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
     sh.copies = mode == TA_PAIR || tile > 64 ? 1 : tile > 32 || mode == TA_WIDE ? 2 : 4;
     sh.whole = (int64_t)a.cache.per_seq * a.cache.page <= TA_WHOLE_BLOCKS * sh.keys;
     if (sh.whole && mode == TA_WIDE) sh.copies = 1;  // no room to join copies in
+    // A CTA that goes on from one unit to the next spends some 5 - 7 us on it, four blocks' time: its run is shorter for that.  (48 sequences of up to 8 drafts
+    // 151.5 -> 146.8 us, 4 x 64 drafts at 30,000 165 -> 156, 1 x 60 at 131,000 295 -> 290.5.  Runs of few blocks would get longer: there it counts nothing.)
+    sh.start = !sh.whole && (int64_t)a.cache.per_seq * a.cache.page / sh.keys * a.cache.seqs * a.cache.G * sh.units_max >= TA_LONG_RUN * sh.ctas ? TA_START : 0;
     return sh;
 }
 // Sums that all segments may leave: one for each unit and one more for each CTA.
