@@ -108,8 +108,9 @@ struct AppendFactors {
         }
     }
 
-    // One head: what was loaded -> what is stored; the whole warp.  head: where it lies (odd halves read the other channels there).
-    __device__ __forceinline__ uint4 apply(const uint4& raw, const bf16* head) const {
+    // One head: what was loaded -> what is stored; the whole warp.  head: where it lies (odd halves read the other channels there, if it `exists`: a warp's last
+    // round may have more places than there are heads).
+    __device__ __forceinline__ uint4 apply(const uint4& raw, const bf16* head, bool exists) const {
         float2 x[4];
         widen(raw, x);
         float inv = 1.f;
@@ -142,8 +143,8 @@ struct AppendFactors {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = first + 2 * e;
-                if (turned(2 * e)) y[e].x = fmaf(to_f32(head[d < half ? d + half : d - half]) * inv, other[e].x, y[e].x);
-                if (turned(2 * e + 1)) y[e].y = fmaf(to_f32(head[d + 1 < half ? d + 1 + half : d + 1 - half]) * inv, other[e].y, y[e].y);
+                if (exists && turned(2 * e)) y[e].x = fmaf(to_f32(head[d < half ? d + half : d - half]) * inv, other[e].x, y[e].x);
+                if (exists && turned(2 * e + 1)) y[e].y = fmaf(to_f32(head[d + 1 < half ? d + 1 + half : d + 1 - half]) * inv, other[e].y, y[e].y);
             }
         }
         return narrow(y);
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(PA_THREADS, 16) paged_append_kernel(const __gr
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 if (u >= left) break;
-                const uint4 y = t.apply(raw[u], src + at);
+                const uint4 y = t.apply(raw[u], src + at, h < heads);
                 if (t.live && h < heads) t.store(q + at, y);
                 h += step, at += far;
             }
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(PA_THREADS, 16) paged_append_kernel(const __gr
         bf16* k = c.k + page * c.k_page + in * c.k_slot;
         int h = head0, at = k_at;
         for (int left = (c.G - warp0 + step - 1) / step; left > 0; --left) {
-            const uint4 y = t.apply(key, src + at);
+            const uint4 y = t.apply(key, src + at, h < c.G);
             if (t.live && h < c.G) t.store(k + h * c.k_head, y);
             h += step, at += far;
             if (t.live && h < c.G) key = t.load(src + at);
