@@ -72,6 +72,7 @@ __device__ __forceinline__ float hl_max_nan(float a, float b) {
     return y;
 }
 __device__ __forceinline__ void hl_tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+    __syncwarp();  // the whole warp's, as every access to tensor memory
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"

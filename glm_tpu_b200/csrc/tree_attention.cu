@@ -43,7 +43,7 @@
 // Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.  A cache of
 // at most four blocks a sequence is dealt in whole units and needs none (JOINS: the copies meet in shared memory, which costs a stage of the ring: 64 pairs
 // at 30,000 slots 109 us so, 103 otherwise): 36 requests of three tokens 22 -> 14.5 us, one token over 12 slots 14 -> 9.8.
-// Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
+// Every wait is bounded and a whole warp's, so that its lanes take one branch; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
 #include "paged.cuh"
 #include "tcgen05.cuh"
 #include "vec8.cuh"
@@ -149,6 +149,7 @@ struct TreeWalk {
 };
 
 __device__ __forceinline__ void ta_tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+    __syncwarp();  // the whole warp's, as every access to tensor memory
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -454,7 +455,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int block = s.block0 + nth(t, n), base = block * KEYS;
                 const uint32_t number = gone + nth(t, n), st = number % STAGES;
                 const uint32_t buffer = T::SCORES == 2 ? seen & 1 : 0, s_addr = tmem + t * 128 + buffer * 64 + lanes;
-                if (!mbar_wait(&s_full[t][buffer], (T::SCORES == 2 ? seen >> 1 : seen) & 1) || fail) { ok = false; break; }
+                if (!mbar_wait_warp(&s_full[t][buffer], (T::SCORES == 2 ? seen >> 1 : seen) & 1) || __any_sync(0xffffffffu, fail)) { ok = false; break; }
                 ++seen;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t there = ~0u;
@@ -490,7 +491,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         m = most;
                     } else if (__any_sync(0xffffffffu, most > m + TA_SLACK)) {
                         if (T::SCORES == 2) {  // the product before this block's may still be adding
-                            if (!__all_sync(0xffffffffu, mbar_wait(pv_done + t, (seen - 2) & 1))) ok = false;
+                            if (!mbar_wait_warp(pv_done + t, (seen - 2) & 1)) ok = false;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         }
                         const float next = fmaxf(m, most), fix = next == -INFINITY ? 1.f : ta_exp2(m - next);
@@ -507,6 +508,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     const float from = m == -INFINITY ? 0.f : m;
                     const float2 scale_2 = make_float2(scale2, scale2), from_2 = make_float2(-from, -from);
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    __syncwarp();  // before the stores
 #pragma unroll
                     for (int w = 0; w < PARTS; ++w) {
                         uint32_t hi[16], lo[16];
@@ -535,7 +537,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 if (drafted && fixes) {  // values that nobody, or not everybody, may multiply
-                    if (!mbar_wait(v_full + st, (number / STAGES) & 1)) { ok = false; break; }
+                    if (!mbar_wait_warp(v_full + st, (number / STAGES) & 1)) { ok = false; break; }
                     const int key = (KEYS / 4) * quarter + lane, draft = base + key - s.seq.length;
                     if (lane < KEYS / 4 && draft >= 0) {
                         unsigned char* at = v_s + st * vboxes * T::KV_BOX + key * 128;
@@ -558,7 +560,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             // the output of the segment: group 0 of a single tile takes what group 1 has along
             if (MODE == TA_SINGLE && t == 1) {
-                if (ok && (used[1] == 0 || mbar_wait(o_free + 1, (used[1] - 1) & 1))) {
+                if (ok && (used[1] == 0 || mbar_wait_warp(o_free + 1, (used[1] - 1) & 1))) {
                     ml_s[row][0] = m, ml_s[row][1] = l;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ml_full);
@@ -570,8 +572,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 continue;
             }
             const bool both = MODE == TA_SINGLE && other > 0;
-            if (ok) ok = mbar_wait(o_full + t, used[t] & 1) && !fail;
-            if (ok && both) ok = mbar_wait(o_full + 1, used[1] & 1) && mbar_wait(&ml_full, joined & 1) && !fail;
+            if (ok) ok = mbar_wait_warp(o_full + t, used[t] & 1) && !__any_sync(0xffffffffu, fail);
+            if (ok && both) ok = mbar_wait_warp(o_full + 1, used[1] & 1) && mbar_wait_warp(&ml_full, joined & 1) && !__any_sync(0xffffffffu, fail);
             ++used[t];
             if (both) ++used[1], ++joined;
             if (!ok) fail = 1;

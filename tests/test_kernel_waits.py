@@ -1,0 +1,27 @@
+"""What the kernels for scoring and for drafted tokens do about waits, read from their sources: a wait that runs out cannot be provoked on a GPU that others share."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "glm_tpu_b200" / "csrc"
+KERNELS = ("tree_attention.cu", "head_logprobs_tcgen05.cu")
+
+
+def code_of(name: str) -> str:
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+
+
+@pytest.mark.parametrize("name", KERNELS)
+def test_waits_are_a_whole_warps(name):
+    """Instructions of the whole warp follow every wait, and a lane whose wait ran out alone would leave the others waiting for it."""
+    code = code_of(name)
+    assert "mbar_wait_warp(" in code and not re.search(r"\bmbar_wait\(", code)
+    assert not re.search(r"(\|\||&& !)\s*fail\b", code)  # nor does a lane decide by itself to leave
+
+
+@pytest.mark.parametrize("name, load", [("tree_attention.cu", "ta_tmem_ld32_nowait"), ("head_logprobs_tcgen05.cu", "hl_tmem_ld32_nowait"), ("tcgen05.cuh", "tmem_ld32"), ("tcgen05.cuh", "tmem_ld16")])
+def test_a_warp_meets_before_it_loads_from_tensor_memory(name, load):
+    body = code_of(name).split(f"void {load}(")[1].split("asm volatile")[0]
+    assert "__syncwarp();" in body
