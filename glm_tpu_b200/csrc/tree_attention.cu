@@ -183,6 +183,13 @@ __device__ __forceinline__ float ta_exp2(float x) {
     return y;
 }
 
+// Whether the condition holds for any of the 128 threads of a group; a barrier of theirs.
+__device__ __forceinline__ bool ta_any_of_group(bool here) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)here) : "memory");
+    return any != 0;
+}
+
 // Bits i of a word of 32 keys whose first lies `ahead` slots behind the first drafted one (negative: before it): committed, or drafted and in the mask.
 __device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
     if (ahead >= 64) return 0u;
@@ -593,7 +600,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int64_t part = sh.part(((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x, MODE == TA_PAIR ? t : 0, JOINS ? 0 : copy);
             if constexpr (JOINS) {  // every copy learns the sums of the row's keys
                 copy_s[row][0] = m, copy_s[row][1] = l;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                ok = !ta_any_of_group(!ok);  // the four warps go on together, or none of them does: those that did would wait for the others without a limit
+                if (!ok) break;
                 float next = m, all = 0.f;
 #pragma unroll
                 for (int k = 0; k < COPIES; ++k) next = fmaxf(next, copy_s[k * T::ROWS + in][0]);
@@ -678,8 +686,6 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (upto < c.vdim) asm volatile("bar.sync 1, 128;" ::: "memory");  // before the next columns
                 }
             }
-            if (JOINS && fail) ok = false;  // all four warps came to the same barriers
-            if (!ok) break;
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {

@@ -25,3 +25,19 @@ def test_waits_are_a_whole_warps(name):
 def test_a_warp_meets_before_it_loads_from_tensor_memory(name, load):
     body = code_of(name).split(f"void {load}(")[1].split("asm volatile")[0]
     assert "__syncwarp();" in body
+
+
+@pytest.mark.parametrize("name", KERNELS)
+def test_who_reads_the_failure_word_decides_for_a_whole_warp(name):
+    """Other warps set it whenever their waits run out: what one warp reads, the next one need not."""
+    code = code_of(name)
+    reads = [code[: m.end()] for m in re.finditer(r"\bfail\b(?! = )", code) if not code[: m.start()].endswith("uint32_t ")]
+    assert reads and all(read.endswith("__any_sync(0xffffffffu, fail") for read in reads), [read[-60:] for read in reads]
+
+
+def test_warps_that_join_copies_leave_together():
+    """Their barrier has no limit, so a segment's first one also decides, for all four, whether there will be a next one."""
+    output = code_of("tree_attention.cu").split("if (!ok && !JOINS) break;")[1].split("mbar_arrive(o_free + t);")[0]
+    first, rest = output.split("ok = !ta_any_of_group(!ok);")
+    assert "bar.sync" not in first and not re.search(r"\bok\b", first) and rest.lstrip().startswith("if (!ok) break;")
+    assert rest.count("bar.sync 1, 128") == 2 and not re.search(r"\bok\b|\bfail\b", rest.split("if (!ok) break;", 1)[1])
