@@ -19,15 +19,19 @@
 // A tile of up to 64 or 32 pairs is there two or four times among the 128 rows: each copy weighs its own half or quarter of every block (its weights of the rest
 // are zeros), so that all threads have a part of the exponentials; the copies' sums meet like those of different runs, or in shared memory.
 //
-// The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  Tiles that share a
-// unit (PAIR) keep both groups of softmax threads busy, and the tensor core: their weights are one bf16 piece, a rounding of 2^-8 each beside that of the
-// result.  What bounds them is one warp that issues for both: a block of 128 keys of two tiles takes 2.7 thousand cycles of softmax (2.0 of them exponentials)
-// and 1.9 until the next scores are there (shared memory feeds S at half the rate of the tensor core).  60 drafts of 8 heads at 131,000 slots: 296 us, 303
-// before the softmax threads got the registers that their scores need (167 -> 157 for 4 x 64 drafts at 30,000).  Measured beside those 303: two buffers of
-// scores, blocks of 64 keys 424 us, with two issuing warps 303; blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
-// A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run; its weights keep a second piece, the
-// remainder of the first (one piece: 108 -> 101 us for 4 x 16 drafts at 30,000).  Heads wider than 128 (WIDE): blocks of 64 keys, one group, and two buffers of
-// scores, so that the next ones are there when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer 320).
+// The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  A weight is two bf16
+// pieces, the second one the remainder of the first, so that 16 bits of it reach the product in every form: a row's digits do not depend on how many rows its call
+// has.  One piece, a rounding of 2^-8 each beside that of the result, took 101 in place of 108 us for 4 x 16 drafts at 30,000 and 287 in place of 365 for 60 at 131,000;
+// its error there was 2.3e-3 of the largest output, where the result's own rounding is 1.7e-3.
+//
+// Tiles that share a unit (PAIR) keep both groups of softmax threads busy, and the tensor core.  What bounds them is one warp that issues for both: a block of 128
+// keys of two tiles takes some 2.7 thousand cycles of softmax (2.0 of them exponentials) and 3.1 of products at the tensor core's own rate
+// (shared memory feeds S at half of it).  60 drafts of 8 heads at 131,000 slots: 365 us.  Measured with one piece, beside 303 (287 since the softmax threads have
+// the registers that their scores need and the start of a unit counts in the runs): two buffers of scores, blocks of 64 keys 424 us, with two issuing warps 303;
+// blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
+// A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run.  Heads wider than 128 (WIDE): blocks of 64 keys,
+// one group, and two buffers of scores, so that the next ones are there when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer
+// 320).
 //
 //   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
 //   warp 8           issues every tcgen05.mma, owns the TMEM allocation
@@ -200,7 +204,7 @@ __device__ __forceinline__ uint32_t ta_visible(int ahead, uint64_t mask) {
 
 template <int MODE, int COPIES, bool JOINS> struct TreeMode {
     static constexpr int KEYS = MODE == TA_WIDE ? 64 : 128, ROWS = 128 / COPIES, COLS = KEYS / COPIES;  // rows of the tile, keys of a block that a thread weighs
-    static constexpr int GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, PIECES = MODE == TA_PAIR ? 1 : 2, SCORES = MODE == TA_WIDE ? 2 : 1;  // buffers
+    static constexpr int GROUPS = MODE == TA_WIDE ? 1 : 2, QTILES = MODE == TA_PAIR ? 2 : 1, SCORES = MODE == TA_WIDE ? 2 : 1;  // buffers
     static constexpr int STAGES = MODE == TA_SINGLE && !JOINS ? 3 : 2, BOXES = MODE == TA_WIDE ? 4 : 2;
     static constexpr int THREADS = MODE == TA_PAIR ? 384 : 352;  // a pair's last warp is there to give its registers away
     static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
@@ -407,7 +411,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const uint32_t p_addr = tmem + t * 128 + buffer * 64;
                 if (elect_one()) {
 #pragma unroll
-                    for (int piece = 0; piece < T::PIECES; ++piece)
+                    for (int piece = 0; piece < 2; ++piece)  // of the weights
 #pragma unroll
                         for (int k = 0; k < KEYS / 16; ++k)
                             umma_bf16_ts(tmem + 256 + t * 128, p_addr + piece * (KEYS / 2) + k * 8, v_at + k * 128, idesc_o, (j > 0 || piece > 0 || k > 0) ? 1u : 0u);
@@ -524,20 +528,18 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                             const float2 z = __ffma2_rn(make_float2(x[w * 32 + 2 * i], x[w * 32 + 2 * i + 1]), scale_2, from_2), p = make_float2(ta_exp2(z.x), ta_exp2(z.y));
                             sum[i & 1] = __fadd2_rn(sum[i & 1], p);
                             hi[i] = pack_bf16(p.x, p.y);
-                            if (T::PIECES == 2) {
-                                const float2 rest = __fadd2_rn(p, make_float2(-bf16_lo(hi[i]), -bf16_hi(hi[i])));
-                                lo[i] = pack_bf16(rest.x, rest.y);
-                            }
+                            const float2 rest = __fadd2_rn(p, make_float2(-bf16_lo(hi[i]), -bf16_hi(hi[i])));
+                            lo[i] = pack_bf16(rest.x, rest.y);
                         }
                         ta_tmem_st16(s_addr + col0 / 2 + w * 16, hi);
-                        if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + col0 / 2 + w * 16, lo);
+                        ta_tmem_st16(s_addr + KEYS / 2 + col0 / 2 + w * 16, lo);
                     }
                     if constexpr (COPIES > 1) {  // the other copies' keys are not this row's
                         const uint32_t none[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
                         for (int at = 0; at < KEYS / 2; at += 16)
                             if (at < col0 / 2 || at >= col0 / 2 + T::COLS / 2) {
                                 ta_tmem_st16(s_addr + at, none);
-                                if (T::PIECES == 2) ta_tmem_st16(s_addr + KEYS / 2 + at, none);
+                                ta_tmem_st16(s_addr + KEYS / 2 + at, none);
                             }
                     }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);

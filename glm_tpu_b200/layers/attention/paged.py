@@ -5,8 +5,10 @@ each sequence's committed ones; ``tree_attention`` lets every drafted token see 
 of a tree.  Tokens that were accepted are appended once more, at consecutive slots (their position, and so their rotation, stays): rows of one call
 are read from the projection and not from the cache, so no slot is moved within it.  A tree of one token is ordinary decoding, a chain a short prompt.
 
-bf16, fp32 sums, one rounding of every result.  Sequences, slots, pages and positions out of range are never followed: they are OR-ed into ``status`` (an
-int32 tensor of one element on the same GPU) as a bad index, the row stores nothing and its queries are zeros; in attention such a slot is not attended to.
+bf16, fp32 sums, one rounding of every result; in the attention a softmax weight meets the values with 16 bits.  Sequences, slots, pages and positions out of
+range are never followed: they are OR-ed into ``status`` (an int32 tensor of one element on the same GPU) as a bad index, the row stores nothing and its queries
+are zeros; in attention such a slot is not attended to.  What a row does not see may hold anything; a NaN or an infinity that it does see makes it NaN there (an
+infinite drafted value: infinite).
 """
 
 from __future__ import annotations
