@@ -17,7 +17,7 @@
 //   warp 1      TMEM allocation; issues the MMAs (of a pair: in the first CTA)
 //   warps 2-9   sums: a thread a row, two warps a quarter of the rows, each half of the tokens
 //
-// Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
+// Every wait is bounded; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT, makes the rows whose sums are missing NaN, and the CTA still releases its TMEM.
 #include "logprobs.cuh"
 #include "tcgen05.cuh"
 
@@ -202,7 +202,7 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
                     }
                     __syncwarp();
                 }
-                if (elect_one()) C::commit(acc_full + acc);  // complete, or abandoned after a timeout: either way release the others
+                if (ok && elect_one()) C::commit(acc_full + acc);  // of a pair the other CTA too takes what is announced for complete: abandoned sums never are
                 __syncwarp();
             }
         }
@@ -216,9 +216,9 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
         kept.clear();
         uint32_t used = 0;
         bool ok = true;
-        int row = -1, token = -1;
+        int row = -1, token = -1, n = 0;
         HeadTile t;
-        for (int n = 0; ok && hl_tile(plan, p.vocab, worker, n, t); ++n) {
+        for (; ok && hl_tile(plan, p.vocab, worker, n, t); ++n) {
             const int now = t.block * ROWS + rank * 128 + quarter * 32 + lane;
             if (now != row) row = now, token = row < p.rows ? lp_token(p.scores, row, p.vocab, false) : -1;
             const int token0 = t.token0 + half * 128, here = t.tokens - half * 128;  // tokens of this half: what lies behind them is of nobody
@@ -304,6 +304,10 @@ __device__ __forceinline__ void head_logprobs_cta(const CUtensorMap& map_a, cons
         if (!ok) {
             fail = 1;
             if (lane == 0) raise_status(p.scores.status, GLMB_STATUS_WAIT_TIMEOUT);
+            do {  // no numbers where sums are missing: NaN in the rows of this tile and of those that will not be taken any more
+                const int lost = t.block * ROWS + rank * 128 + quarter * 32 + lane;
+                if (lost < p.rows) p.part[(int64_t)lost * plan.parts + t.part * 2 + half] = make_float4(INFINITY, __int_as_float(0x7fffffff), 0.f, 0.f);
+            } while (!plan.keeps && hl_tile(plan, p.vocab, worker, ++n, t));
         } else if (plan.keeps && row >= 0 && row < p.rows) {
             p.part[(int64_t)row * plan.parts + t.part * 2 + half] = make_float4(kept.m, kept.s, kept.t, 0.f);
         }

@@ -41,3 +41,11 @@ def test_warps_that_join_copies_leave_together():
     first, rest = output.split("ok = !ta_any_of_group(!ok);")
     assert "bar.sync" not in first and not re.search(r"\bok\b", first) and rest.lstrip().startswith("if (!ok) break;")
     assert rest.count("bar.sync 1, 128") == 2 and not re.search(r"\bok\b|\bfail\b", rest.split("if (!ok) break;", 1)[1])
+
+
+def test_sums_that_a_lost_wait_leaves_out_are_no_numbers():
+    """The status word may be nobody's: what was not summed up must not be read as if it had been."""
+    code = code_of("head_logprobs_tcgen05.cu")
+    assert code.count("C::commit(acc_full + acc)") == 1 and "if (ok && elect_one()) C::commit(acc_full + acc);" in code  # abandoned sums are not announced
+    lost = code.split("GLMB_STATUS_WAIT_TIMEOUT);")[1].split("} else if (plan.keeps")[0]
+    assert "p.part[" in lost and "__int_as_float(0x7fffffff)" in lost and "while (!plan.keeps && hl_tile(" in lost
