@@ -47,7 +47,8 @@
 // Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.  A cache of
 // at most four blocks a sequence is dealt in whole units and needs none (JOINS: the copies meet in shared memory, which costs a stage of the ring: 64 pairs
 // at 30,000 slots 109 us so, 103 otherwise): 36 requests of three tokens 22 -> 14.5 us, one token over 12 slots 14 -> 9.8.
-// Every wait is bounded and a whole warp's, so that its lanes take one branch; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT and the CTA still releases its TMEM.
+// Every wait is bounded and a whole warp's, so that its lanes take one branch; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT, makes the rows
+// whose sums are missing NaN, and the CTA still releases its TMEM.
 #include "paged.cuh"
 #include "tcgen05.cuh"
 #include "vec8.cuh"
@@ -210,7 +211,32 @@ template <int MODE, int COPIES, bool JOINS> struct TreeMode {
     static constexpr int Q_BOX = 128 * 128, KV_BOX = KEYS * 128;  // bytes of a box of 64 columns
     static constexpr int JOIN = JOINS ? 128 * TA_JOIN * 4 : 0;  // 64 columns of the copies' sums
     static constexpr int SMEM = QTILES * BOXES * Q_BOX + 2 * STAGES * BOXES * KV_BOX + JOIN + 1024;
+
+    // Of group t in a segment: its tile, whether nobody else has keys of the tile's rows, and else where their sums go.
+    static __device__ __forceinline__ int tile_of(const TreeShape& sh, const TreeSegment& s, int t) { return s.unit * sh.in_unit + (MODE == TA_PAIR ? t : 0); }
+    static __device__ __forceinline__ bool alone(const TreeSegment& s) { return (JOINS || COPIES == 1) && s.blocks == s.of; }
+    static __device__ __forceinline__ int64_t part_of(const TreeAttentionArgs& a, const TreeShape& sh, const TreeSegment& s, int t, int copy) {
+        return sh.part(((int64_t)s.b * a.cache.G + s.g) * sh.units_max + s.unit + blockIdx.x, MODE == TA_PAIR ? t : 0, JOINS ? 0 : copy);
+    }
 };
+
+// After a lost wait: no numbers where sums are missing.  NaN in the thread's row of this segment and of those that will not be taken any more.
+template <int MODE, int COPIES, bool JOINS>
+__device__ __noinline__ void tree_lost(const TreeAttentionArgs& a, const TreeShape& sh, TreeWalk walk, TreeSegment s, int t, int row) {
+    typedef TreeMode<MODE, COPIES, JOINS> T;
+    const int copy = row / T::ROWS, in = row % T::ROWS;
+    const float none = __int_as_float(0x7fffffff);
+    do {
+        const int tile = T::tile_of(sh, s, t), j = tile / sh.head_blocks * sh.tile_rows + in / sh.heads, hh = tile % sh.head_blocks * sh.heads + in % sh.heads;
+        if (in >= sh.heads * sh.tile_rows || tile >= sh.tiles(s.seq.rows) || j >= s.seq.rows || hh >= sh.per || (JOINS && copy)) continue;
+        if (!T::alone(s)) {  // the launch that joins them sees it
+            *reinterpret_cast<float2*>(a.part_ml + (T::part_of(a, sh, s, t, copy) + in) * 2) = make_float2(none, none);
+            continue;
+        }
+        bf16* dst = a.out + (int64_t)(s.seq.row0 + j) * a.out_row + (int64_t)(s.g * sh.per + hh) * a.out_head;
+        for (int x = 0; x < a.cache.vdim; x += 8) *reinterpret_cast<uint4*>(dst + x) = make_uint4(~0u, ~0u, ~0u, ~0u);
+    } while (walk.next(a, sh, s));
+}
 
 template <int MODE, int COPIES, bool JOINS>
 __global__ void __launch_bounds__(TreeMode<MODE, COPIES, JOINS>::THREADS, 1)
@@ -456,7 +482,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (other) ++used[1 - t];
                 continue;
             }
-            const int tile = s.unit * sh.in_unit + (MODE == TA_PAIR ? t : 0), j0 = tile / sh.head_blocks * sh.tile_rows, h0 = tile % sh.head_blocks * sh.heads;
+            const int tile = T::tile_of(sh, s, t), j0 = tile / sh.head_blocks * sh.tile_rows, h0 = tile % sh.head_blocks * sh.heads;
             const int j = j0 + in / sh.heads, hh = h0 + in % sh.heads;
             const bool live = in < sh.heads * sh.tile_rows && j < s.seq.rows && hh < sh.per, warp_live = __any_sync(0xffffffffu, live);
             const uint64_t drafts = s.seq.drafts >= 64 ? ~0ull : (1ull << s.seq.drafts) - 1ull;
@@ -589,7 +615,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (!ok && !JOINS) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t lost = broken[segment & 3] & mask;
-            const bool whole = (JOINS || COPIES == 1) && s.blocks == s.of;  // nobody else has keys of this row
+            const bool whole = T::alone(s);  // nobody else has keys of this row
             float f0 = 1.f, f1 = 0.f;
             if (both) {
                 const float m1 = ml_s[row][0], l1 = ml_s[row][1], next = fmaxf(m, m1);
@@ -599,7 +625,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 m = isnan(m1) ? m1 : next;
             }
             const int head = s.g * sh.per + hh, out_row = s.seq.row0 + j;
-            const int64_t part = sh.part(((int64_t)s.b * c.G + s.g) * sh.units_max + s.unit + blockIdx.x, MODE == TA_PAIR ? t : 0, JOINS ? 0 : copy);
+            const int64_t part = T::part_of(a, sh, s, t, copy);
             if constexpr (JOINS) {  // every copy learns the sums of the row's keys
                 copy_s[row][0] = m, copy_s[row][1] = l;
                 ok = !ta_any_of_group(!ok);  // the four warps go on together, or none of them does: those that did would wait for the others without a limit
@@ -698,6 +724,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (!ok) {
             fail = 1;
             if (lane == 0) raise_status(a.status, GLMB_STATUS_WAIT_TIMEOUT);
+            if (MODE != TA_SINGLE || t == 0) tree_lost<MODE, COPIES, JOINS>(a, sh, walk, s, t, quarter * 32 + lane);
         }
         if (sh.whole && a.clear_rest)  // there is no second launch
             for (int r = blockIdx.x * 8 + warp; r < a.rows; r += gridDim.x * 8) {

@@ -49,3 +49,8 @@ def test_sums_that_a_lost_wait_leaves_out_are_no_numbers():
     assert code.count("C::commit(acc_full + acc)") == 1 and "if (ok && elect_one()) C::commit(acc_full + acc);" in code  # abandoned sums are not announced
     lost = code.split("GLMB_STATUS_WAIT_TIMEOUT);")[1].split("} else if (plan.keeps")[0]
     assert "p.part[" in lost and "__int_as_float(0x7fffffff)" in lost and "while (!plan.keeps && hl_tile(" in lost
+    code = code_of("tree_attention.cu")
+    after = code.split("raise_status(a.status, GLMB_STATUS_WAIT_TIMEOUT);")[1].split("if (sh.whole && a.clear_rest)")[0]
+    assert "if (MODE != TA_SINGLE || t == 0) tree_lost<MODE, COPIES, JOINS>(a, sh, walk, s, t, quarter * 32 + lane);" in after  # the group that stores the output
+    lost = code.split("void tree_lost(")[1].split("while (walk.next(a, sh, s));")[0]
+    assert "make_float2(none, none)" in lost and "make_uint4(~0u, ~0u, ~0u, ~0u)" in lost
