@@ -11,7 +11,7 @@ is printed.
 
 An entry with ``"score"`` instead of ``want`` has its tokens scored: ``{"id": "a", "tokens": [5, 17, 3], "score": {"top": 2, "next": 9}}`` asks at every
 place for the log probability of the token that comes after it (``next``, which may be left out, after the last) and for the ``top`` most likely ones
-(0 to 32; left out: none).  The scores of a step go to ``<out>/<step>.scores.json``, a list with an object for every scored entry: ``id``,
+(0 to 32, and no more than there are; left out: none).  The scores of a step go to ``<out>/<step>.scores.json``, a list with an object for every scored entry: ``id``,
 ``logprob``, ``entropy`` and ``best`` (the most likely token's log probability), a number a place (null: nothing was asked there, or the place has no probabilities), and
 ``top``, ``[token, log probability]`` pairs a place.  Natural logarithms; minus infinity is written as -Infinity.
 
@@ -34,13 +34,15 @@ LANES = 4
 PREFILL_CHUNK = 2048
 
 
-def _check_score(entry: dict) -> None:
+def _check_score(entry: dict, vocab: int) -> None:
     asked = entry["score"]
     if not isinstance(asked, dict) or set(asked) - {"top", "next"} or entry.get("want"):
         raise RequestValidationError("an entry is scored with top and next, and has no wanted places then")
     top, following = asked.get("top", 0), asked.get("next", 0)
-    if type(top) is not int or not 0 <= top <= 32 or type(following) is not int or following < 0:
-        raise RequestValidationError("top is between 0 and 32, next a token id")
+    if type(top) is not int or not 0 <= top <= min(32, vocab):
+        raise RequestValidationError(f"top is between 0 and {min(32, vocab)}")
+    if not entry["tokens"] or any(type(t) is not int or not 0 <= t < vocab for t in (*entry["tokens"], following)):
+        raise RequestValidationError("scored tokens, of which there is at least one, and next are token ids of the model")
 
 
 def _scores_of(name: str, scores) -> dict:
@@ -53,10 +55,11 @@ def _scores_of(name: str, scores) -> dict:
 
 class TraceReplay:
     """Requests by name on the lanes of a runner.  The runner needs ``lanes``, ``lengths``, ``open_lane``, ``extend`` and ``decode_logits``, and ``score``
-    for entries that are scored."""
+    for entries that are scored; what those ask for is checked against the vocabulary of its geometry ``g``, if it has one, before a step begins."""
 
     def __init__(self, runner):
         self.runner = runner
+        self.vocab = runner.g.vocab_size if hasattr(runner, "g") else 1 << 31
         self.scores: list[dict] = []  # of the last step
         self.free = list(range(runner.lanes))
         self.lane_of: dict[str, int] = {}
@@ -77,7 +80,7 @@ class TraceReplay:
             raise RequestValidationError("a request has two entries in one step")
         for entry in entries:
             if "score" in entry:
-                _check_score(entry)
+                _check_score(entry, self.vocab)
         self.scores = []
         lanes = [self._lane(name) for name in names]
         single = {lane: e["tokens"][0] for lane, e in zip(lanes, entries) if len(e["tokens"]) == 1 and self.runner.lengths[lane] > 0 and "score" not in e}

@@ -276,7 +276,8 @@ class LaneRunner:
     def score(self, lane: int, token_ids, *, following: int | None = None, top: int = 0):
         """Run the next tokens of ``lane`` through the prefill program as ``extend`` does and score them: place ``i`` is asked for the token
         at ``i + 1``, the last place for ``following`` (without one its log probability is NaN).  Returns ``TokenLogprobs`` on the CPU, with the
-        ``top`` most likely tokens of every place where asked for.  The logits are those of the family in fp32, not rounded, and are not kept."""
+        ``top`` most likely tokens of every place where asked for.  The logits are those of the family in fp32, not rounded, and are not kept.
+        Token ids outside the vocabulary are refused before anything runs."""
         from glm_tpu_b200.layers import logprobs
         from glm_tpu_b200.layers.contracts import TokenLogprobs
 
@@ -287,11 +288,14 @@ class LaneRunner:
             raise ValueError("the tokens do not fit the context capacity")
         if not 0 <= top <= min(logprobs.MAX_TOP, self.g.vocab_size):
             raise ValueError(f"between 0 and {min(logprobs.MAX_TOP, self.g.vocab_size)} alternatives")
+        ids = list(token_ids)
+        if min(ids) < 0 or max(ids) >= self.g.vocab_size or (following is not None and not 0 <= following < self.g.vocab_size):
+            raise ValueError(f"token ids are between 0 and {self.g.vocab_size - 1}")
         parts = []
         with torch.cuda.device(self.device):
-            asked = _host_ids([*list(token_ids)[1:], -1 if following is None else following]).pin_memory().to(self.device, non_blocking=True)
+            asked = _host_ids([*ids[1:], -1 if following is None else following]).pin_memory().to(self.device, non_blocking=True)
             status = torch.zeros(1, dtype=torch.int32, device=self.device)
-            for start, hidden in self._chunks(lane, token_ids, first, lambda start, rows: slice(0, rows), head="hidden"):
+            for start, hidden in self._chunks(lane, ids, first, lambda start, rows: slice(0, rows), head="hidden"):
                 step = SCORED_ROWS if top else hidden.shape[0]  # rows whose logits are in memory at once: none without alternatives
                 for r in range(0, hidden.shape[0], step):
                     x, k = hidden[r : r + step], asked[start + r : start + min(r + step, hidden.shape[0])]
