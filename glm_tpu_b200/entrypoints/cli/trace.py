@@ -13,7 +13,7 @@ An entry with ``"score"`` instead of ``want`` has its tokens scored: ``{"id": "a
 place for the log probability of the token that comes after it (``next``, which may be left out, after the last) and for the ``top`` most likely ones
 (0 to 32, and no more than there are; left out: none).  The scores of a step go to ``<out>/<step>.scores.json``, a list with an object for every scored entry: ``id``,
 ``logprob``, ``entropy`` and ``best`` (the most likely token's log probability), a number a place (null: nothing was asked there, or the place has no probabilities), and
-``top``, ``[token, log probability]`` pairs a place.  Natural logarithms; minus infinity is written as -Infinity.
+``top``, ``[token, log probability]`` pairs a place (``[-1, null]`` where it has no probabilities).  Natural logarithms; minus infinity is written as -Infinity.
 
 The requests run on the engine's own lanes: a request's later single tokens go through the decode program's kernels (those of one step
 together, one lane each), everything else through the prefill program, both from the cache that earlier steps left.

@@ -277,9 +277,11 @@ class LaneRunner:
         """Run the next tokens of ``lane`` through the prefill program as ``extend`` does and score them: place ``i`` is asked for the token
         at ``i + 1``, the last place for ``following`` (without one its log probability is NaN).  Returns ``TokenLogprobs`` on the CPU, with the
         ``top`` most likely tokens of every place where asked for.  The logits are those of the family in fp32, not rounded, and are not kept.
-        Token ids outside the vocabulary are refused before anything runs."""
+        A place whose logits have a NaN or plus infinity has no probabilities: NaN, and ids of -1.  Token ids outside the vocabulary are refused before
+        anything runs."""
         from glm_tpu_b200.layers import logprobs
         from glm_tpu_b200.layers.contracts import TokenLogprobs
+        from glm_tpu_b200.ops import native
 
         n, first = len(token_ids), self.lengths[lane]
         if self.world > 1:
@@ -307,9 +309,9 @@ class LaneRunner:
             self.state.positions[lane].fill_(first + n)
             scores = TokenLogprobs(*(torch.cat(column).cpu() if column[0] is not None else None for column in zip(*(vars(p).values() for p in parts))))
             self.peer.check_status()
-            bits = int(status)
+            bits = int(status) & ~native.STATUS_NONFINITE  # which the scores say themselves
             if bits:
-                raise DeviceStatusError("device status: a scored token lies outside the vocabulary, or a place has no finite logits", bits)
+                raise DeviceStatusError("device status: the scores are not complete", bits)
         return scores
 
     def decode_logits(self, tokens: dict) -> dict:
