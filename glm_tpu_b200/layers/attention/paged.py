@@ -48,6 +48,11 @@ def ancestor_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
     return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64), torch.tensor(depths, dtype=torch.int32)
 
 
+def _shared(t: torch.Tensor) -> bool:
+    """Whether rows of channels along an axis begin closer together than one is long (``expand``: all at one place)."""
+    return any(n > 1 and step < t.shape[-1] for n, step in zip(t.shape[:-1], t.stride()))
+
+
 def _checked(cache: PagedKV, device: int) -> tuple[int, ...]:
     """The cache as the kernels take it (the fields of ``native.PagedArgs``; the last seven: sequences, their pages, pages, slots of a page, heads, dim, vdim).
     ``device``: where the rows lie (-1: CPU)."""
@@ -66,6 +71,8 @@ def _checked(cache: PagedKV, device: int) -> tuple[int, ...]:
         raise ValueError("rows, pools and table lie on one device")
     if not 16 <= dim <= 256 or not 16 <= vdim <= 256 or dim % 16 or vdim % 16:
         raise ValueError("heads are 16 to 256 channels wide, in multiples of 16")
+    if (k_page < dim or k_slot < dim or k_head < dim or v_page < vdim or v_slot < vdim or v_head < vdim) and (_shared(k) or _shared(v)):
+        raise ValueError("pages, slots and heads of the pools do not share memory")
     k_at, v_at = k.data_ptr(), v.data_ptr()
     if device >= 0 and (k_last != 1 or v_last != 1 or (k_page | k_slot | k_head | v_page | v_slot | v_head) % 8 or (k_at | v_at) % 16):
         raise ValueError("the channels of a head are contiguous and every head of the pools 16-byte aligned")
@@ -149,6 +156,11 @@ def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, length
     if device < 0:
         out = torch.zeros((rows, heads, vdim), dtype=torch.bfloat16) if out is None else out
         return scoring.tree_attention(q, cache.k, cache.v, cache.table, starts, lengths, masks, scale, max_rows, sink, out)
+    row, head, _ = q.stride()
+    if (row < dim or head < dim) and _shared(q):  # a tensor map holds heads that lie apart
+        q = q.contiguous()
+    if out is not None and _shared(out):
+        raise ValueError("rows and heads of out do not share memory")
     for t in (q,) if out is None else (q, out):
         row, head, last = t.stride()
         if last != 1 or (row | head) % 8 or t.data_ptr() % 16:

@@ -65,6 +65,10 @@ def head_logprobs(hidden: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor
     if width % 8 or hidden.stride(1) != 1 or head.stride(1) != 1 or hidden.stride(0) % 8 or head.stride(0) % 8 or (hidden.data_ptr() | head.data_ptr()) % 16:
         raise ValueError("rows of hidden states and table are contiguous, 16-byte aligned and a multiple of 8 wide")
     with native.on_device(hidden):
+        if rows > 1 and hidden.stride(0) < width:  # rows that share memory (``expand``): a tensor map holds rows that lie apart
+            hidden = hidden.contiguous()
+        if vocab > 1 and head.stride(0) < width:
+            head = head[:vocab].contiguous()
         sums = hidden.new_empty((3, rows), dtype=torch.float32)
         native.head_logprobs(hidden, head, vocab, tokens.contiguous(), sums, status=status)
     return TokenLogprobs(*sums.unbind(0), None, None)
