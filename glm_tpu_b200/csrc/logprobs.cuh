@@ -23,18 +23,18 @@ __device__ __forceinline__ float lp_exp2(float x) {  // results below 2^-126 are
 struct LogitSums {
     float m, s, t;
     __device__ __forceinline__ void clear() { m = -INFINITY, s = 0.f, t = 0.f; }
-    __device__ __forceinline__ void join(const LogitSums& o) {
-        const bool mine = m >= o.m;
+    __device__ __forceinline__ void join(const LogitSums& o, bool first = true) {  // first: of two equal maxima this one is kept
+        const bool mine = first ? m >= o.m : m > o.m;
         const float hm = mine ? m : o.m, hs = mine ? s : o.s, ht = mine ? t : o.t, lm = mine ? o.m : m, ls = mine ? o.s : s, lt = mine ? o.t : t;
         const float d = lm - hm, f = lm == -INFINITY ? 0.f : lp_exp2(d * LP_LOG2E), sum = 1.f + ls;
         m = hm;
         s = fmaf(sum, f, hs);
         t = ht + (f > 0.f ? fmaf(sum, d, lt) * f : 0.f);  // d may be minus infinity
     }
-    __device__ __forceinline__ void join_lanes(int lanes) {  // of a warp's first `lanes` (a power of two): the same result on each
+    __device__ __forceinline__ void join_lanes(int lanes) {  // of a warp's first `lanes` (a power of two): the same result, to the bit, on each
         for (int o = lanes >> 1; o > 0; o >>= 1) {
             const LogitSums other{__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), __shfl_xor_sync(0xffffffffu, t, o)};
-            join(other);
+            join(other, (threadIdx.x & o) == 0);
         }
     }
     __device__ __forceinline__ bool bad() const { return isnan(s) || m == INFINITY; }
