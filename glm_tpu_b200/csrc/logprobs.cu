@@ -5,8 +5,9 @@
 // likely tokens: every warp keeps a sorted list, one entry a lane, of 64-bit keys (the logit's order above the id's complement: ties go to the lowest id), and a
 // logit enters only if it reaches a bound that n of the CTA's logits reach: the n-th largest of the threads' maxima so far, found anew after 1, 3, 9, 33 ..
 // stages, at 3.3 thousand clocks.  Of 131,072 logits some 150 enter for n = 20, at 900 clocks.  (With a bound for each warp it was ten times as many.)  Sums and
-// lists meet in the CTA, then in the cluster's first.  2,048 rows of 131,072 fp32 logits, 20 alternatives: 167 us, 6.4 TB/s, the bytes their bound; 333 rows of
-// 65,521, five: 28.5 us, 18.7 without alternatives.
+// lists meet in the CTA, then in the cluster's first.  2,048 rows of 131,072 fp32 logits: 157 us without alternatives, 168 with one (6.4 TB/s, the bytes their
+// bound), 197 with twenty; bf16 113, 145, 188.  333 rows of 65,521, five: 28.5 us, 18.7 without alternatives.  Where fewer of a CTA's logits than alternatives are
+// above minus infinity the bound keeps none away, and every masked one is offered: the 2,048 rows with five tokens left and twenty alternatives take 5.7 ms.
 //
 // A row with a NaN or an infinite logit above zero has no probabilities: its numbers are NaN, its ids -1, and GLMB_STATUS_NONFINITE is raised.  A row
 // of minus infinities alone (its mask leaves nothing): log probabilities minus infinity, entropy 0, the lowest ids.  A token of -1 asks for nothing

@@ -11,7 +11,7 @@
 // weights and angles become two factors a channel, once for the row's q and once for its k, so that a normalized head costs two packed instructions for a
 // pair of channels.  Of a rotation by halves a thread has four channels and the four that they turn with, so that nothing is exchanged.  The first heads and
 // values are on their way before the row's place in the cache is known.  8,191 rows of 64 + 8 + 8 heads of 128: turned by pairs 69.5 us, 4.8 TB/s, by
-// halves 67, neither norm nor turn 55.  Bound: what a row costs before its heads do.  A CTA of 64 threads takes 18 rounds of heads with the same factors (256
+// halves 68.6, neither norm nor turn 56, by odd halves (90 channels; their partners are read once more) 157.  Bound: what a row costs before its heads do.  A CTA of 64 threads takes 18 rounds of heads with the same factors (256
 // threads and 5 rounds 78; 128 threads 71.5), 16 of them an SM (20, with fewer registers: 83); the angles' loads go out with the table's and wait for no
 // branch (behind the page's 85).  Rows in turn, the next one's place looked up ahead, 94; a ring of bulk copies 192.
 #include "paged.cuh"

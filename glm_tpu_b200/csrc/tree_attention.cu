@@ -21,16 +21,16 @@
 //
 // The maximum is only followed when it grows by more than 2^8 (the weights stay finite, the division at the end removes the difference).  A weight is two bf16
 // pieces, the second one the remainder of the first, so that 16 bits of it reach the product in every form: a row's digits do not depend on how many rows its call
-// has.  One piece, a rounding of 2^-8 each beside that of the result, took 101 in place of 108 us for 4 x 16 drafts at 30,000 and 287 in place of 365 for 60 at 131,000;
+// has.  One piece, a rounding of 2^-8 each beside that of the result, took 101 in place of 108 us for 4 x 16 drafts at 30,000 and 287 in place of 369 for 60 at 131,000;
 // its error there was 2.3e-3 of the largest output, where the result's own rounding is 1.7e-3.
 //
 // Tiles that share a unit (PAIR) keep both groups of softmax threads busy, and the tensor core.  What bounds them is one warp that issues for both: a block of 128
 // keys of two tiles takes some 2.7 thousand cycles of softmax (2.0 of them exponentials) and 3.1 of products at the tensor core's own rate
-// (shared memory feeds S at half of it).  60 drafts of 8 heads at 131,000 slots: 365 us.  Measured with one piece, beside 303 (287 since the softmax threads have
+// (shared memory feeds S at half of it).  60 drafts of 8 heads at 131,000 slots: 369 us, tensor pipe active 57 %.  Measured with one piece, beside 303 (287 since the softmax threads have
 // the registers that their scores need and the start of a unit counts in the runs): two buffers of scores, blocks of 64 keys 424 us, with two issuing warps 303;
 // blocks of 128 with two issuing warps 357; exponentials of the two groups in turns 346.
 // A tile alone has the two groups take alternate blocks, each with its own sums, which meet at the end of the run.  Heads wider than 128 (WIDE): blocks of 64 keys,
-// one group, and two buffers of scores, so that the next ones are there when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 267 us, with one buffer
+// one group, and two buffers of scores, so that the next ones are there when a softmax ends (40 drafts of 4 heads of 192 at 100,000 slots: 258 us, with one buffer
 // 320).
 //
 //   warps 0-3, 4-7   softmax and output of group 0 and 1 (warp w reads TMEM lanes 32 (w % 4) ..)
@@ -46,7 +46,7 @@
 //
 // Runs that share a unit, and copies, leave their sums in memory; a second launch joins them, and clears the rows of no sequence where asked to.  A cache of
 // at most four blocks a sequence is dealt in whole units and needs none (JOINS: the copies meet in shared memory, which costs a stage of the ring: 64 pairs
-// at 30,000 slots 109 us so, 103 otherwise): 36 requests of three tokens 22 -> 14.5 us, one token over 12 slots 14 -> 9.8.
+// at 30,000 slots 109 us so, 103 otherwise): 36 requests of three tokens over 12 slots, 16 heads, 18.2 -> 14.1 us, one token of 8 heads of 64 13.2 -> 9.4.
 // Every wait is bounded and a whole warp's, so that its lanes take one branch; one that runs out raises GLMB_STATUS_WAIT_TIMEOUT, makes the rows
 // whose sums are missing NaN, and the CTA still releases its TMEM.
 #include "paged.cuh"
@@ -819,7 +819,8 @@ static TreeShape tree_shape(const TreeAttentionArgs& a, int& mode) {
     sh.whole = (int64_t)a.cache.per_seq * a.cache.page <= TA_WHOLE_BLOCKS * sh.keys;
     if (sh.whole && mode == TA_WIDE) sh.copies = 1;  // no room to join copies in
     // A CTA that goes on from one unit to the next spends some 5 - 7 us on it, four blocks' time: its run is shorter for that.  (48 sequences of up to 8 drafts
-    // 151.5 -> 146.8 us, 4 x 64 drafts at 30,000 165 -> 156, 1 x 60 at 131,000 295 -> 290.5.  Runs of few blocks would get longer: there it counts nothing.)
+    // 151.5 -> 146.8 us; with weights of one piece 4 x 64 drafts at 30,000 165 -> 156 and 1 x 60 at 131,000 295 -> 290.5.  Runs of few blocks would get longer: there
+    // it counts nothing.)  By the table's width: the host does not know the lengths.
     sh.start = !sh.whole && (int64_t)a.cache.per_seq * a.cache.page / sh.keys * a.cache.seqs * a.cache.G * sh.units_max >= TA_LONG_RUN * sh.ctas ? TA_START : 0;
     return sh;
 }

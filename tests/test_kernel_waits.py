@@ -1,4 +1,4 @@
-"""What the kernels for scoring and for drafted tokens do about waits, read from their sources: a wait that runs out cannot be provoked on a GPU that others share."""
+"""What the kernels for scoring and for drafted tokens do about waits, read from their sources: no input makes a wait run out."""
 
 import re
 from pathlib import Path
