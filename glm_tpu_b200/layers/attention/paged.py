@@ -7,8 +7,8 @@ are read from the projection and not from the cache, so no slot is moved within 
 
 bf16, fp32 sums, one rounding of every result; in the attention a softmax weight meets the values with 16 bits.  Sequences, slots, pages and positions out of
 range are never followed: they are OR-ed into ``status`` (an int32 tensor of one element on the same GPU) as a bad index, the row stores nothing and its queries
-are zeros; in attention such a slot is not attended to.  What a row does not see may hold anything; a NaN or an infinity that it does see makes it NaN there (an
-infinite drafted value: infinite).
+are zeros; in attention such a slot is not attended to.  What a row does not see may hold anything.  A committed value that is not finite leaves its channel so, as a
+NaN or an infinity, in the rows of its sequence and in no other.
 """
 
 from __future__ import annotations
@@ -159,10 +159,10 @@ def tree_attention(q: torch.Tensor, cache: PagedKV, starts: torch.Tensor, length
     row, head, _ = q.stride()
     if (row < dim or head < dim) and _shared(q):  # a tensor map holds heads that lie apart
         q = q.contiguous()
-    if out is not None and _shared(out):
-        raise ValueError("rows and heads of out do not share memory")
     for t in (q,) if out is None else (q, out):
         row, head, last = t.stride()
+        if t is out and (row < vdim or head < vdim) and _shared(out):
+            raise ValueError("rows and heads of out do not share memory")
         if last != 1 or (row | head) % 8 or t.data_ptr() % 16:
             raise ValueError("the channels of a head are contiguous and every head of q and out 16-byte aligned")
     with native.on_device(q):
